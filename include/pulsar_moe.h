@@ -61,6 +61,17 @@ extern "C" {
 #define PULSAR_ACT_SILU        0u /* silu(g) * u */
 #define PULSAR_ACT_SWIGLU_OAI  2u /* gpt-oss: clamp 7, alpha 1.702, (u + 1) */
 
+/* act codes of the dense product's epilogue (pulsar_matmul_kq_fused) */
+#define PULSAR_EPI_NONE    0u
+#define PULSAR_EPI_SILU    1u /* v / (1 + exp(-v)) */
+#define PULSAR_EPI_GELU    2u /* v / 2 (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
+#define PULSAR_EPI_RELU    3u /* max(v, 0) */
+#define PULSAR_EPI_SIGMOID 4u /* 1 / (1 + exp(-v)) */
+
+/* scores of pulsar_router_select_groups */
+#define PULSAR_SCORE_SIGMOID 0u
+#define PULSAR_SCORE_SOFTMAX 1u
+
 #define PULSAR_QK_K 256u
 
 /* q8_K activation block (pulsar_kernels.cu:1492-1496; lane Q8KRow,
@@ -110,6 +121,22 @@ int pulsar_quantize_q8_K(void *out, const void *x, uint32_t in_dim, uint32_t n_r
 int pulsar_matmul_kq(void *out, const void *w, const void *xq, uint32_t in_dim,
                      uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes,
                      uint32_t quant);
+
+/* pulsar_matmul_kq with its epilogue in the same launch (no reference
+ * counterpart: the reference runs the bias, the activation and the residual
+ * add as kernels of their own):
+ *   out[t][r] = act(dot(w row r, xq[t]) + bias[r]) + residual[t][r]
+ * bias f32 [out_dim] and residual f32 rows are left out where NULL; act: a
+ * PULSAR_EPI_* code. Row t of out starts at t * out_stride floats, of residual
+ * at t * res_stride (0: out_dim, the packed rows; never less than out_dim);
+ * floats between the rows are left as they are. residual may be out itself, at
+ * the same stride (each element is read before it is written); any other
+ * overlap of out with an operand is refused. The dots are pulsar_matmul_kq's,
+ * bit for bit, with its formats and limits. */
+int pulsar_matmul_kq_fused(void *out, const void *w, const void *xq, const void *bias,
+                           const void *residual, uint32_t in_dim, uint32_t out_dim,
+                           uint32_t n_tok, uint64_t row_bytes, uint32_t quant, uint32_t act,
+                           uint64_t out_stride, uint64_t res_stride);
 
 /* mid[t][s][r] = glu(gate_r . x_t + gate_b[r], up_r . x_t + up_b[r], act_op) * weights[t][s].
  * ptrs: pulsar_expert_ptrs[n_tok][n_used]; weights: f32 [n_tok][n_used];
@@ -188,6 +215,33 @@ int pulsar_router_select(void *selected, void *weights, const void *logits,
                          float weight_scale, uint32_t n_tok, uint32_t softmax_mode,
                          uint32_t n_shexp);
 
+/* Routing with expert groups (no reference counterpart). Per token, of its
+ * logits f32 [n_expert]:
+ *   score s: PULSAR_SCORE_SIGMOID 1 / (1 + exp(-l)), PULSAR_SCORE_SOFTMAX the
+ *     softmax over the token's experts; +-inf beyond f32 counts as the largest
+ *     finite value
+ *   choice c = s + bias[e] (bias f32 [n_expert], NULL: s alone). A logit or
+ *     bias of NaN or -inf takes its expert out of the choice (the logit out of
+ *     the softmax too)
+ *   groups: n_group groups of n_expert / n_group neighbouring experts; a group
+ *     stands with the sum of its group_top (1 or 2) largest c (with one alone
+ *     if it has no other); the topk_group best groups are kept, ties to the
+ *     lower group. n_group = 1: every expert
+ *   selected int32 [n_tok][k_used]: the largest c of the kept groups in
+ *     falling order, ties to the lower id, each expert once; -1 with weight 0
+ *     where fewer than k_used are left
+ *   weights f32 [n_tok][k_used]: the winners' s (without the bias); renorm != 0:
+ *     over their sum (sigmoid: at least 2^-14, as pulsar_router_select); times
+ *     weight_scale
+ * Ids are decided as c stands in 64 bits, whatever f32 would round it to.
+ * n_expert <= 1024, a multiple of n_group <= 64; k_used <= 64 and <= the
+ * experts of topk_group groups. */
+int pulsar_router_select_groups(void *selected, void *weights, const void *logits,
+                                const void *bias, uint32_t n_expert, uint32_t k_used,
+                                uint32_t n_group, uint32_t topk_group, uint32_t group_top,
+                                uint32_t score, uint32_t renorm, float weight_scale,
+                                uint32_t n_tok);
+
 /* out[t][o] = sum_i w[o][i] * x[t][i] in fp32 (router logits). Replaces
  * pulsar_matmul_f32 (pulsar_kernels.cu:6526). */
 int pulsar_matmul_f32(void *out, const void *w, const void *x, uint32_t in_dim,
@@ -244,6 +298,25 @@ int pulsar_moe_route_ptrs(void *ptrs, void *slot_weights, const void *selected,
  * n_tok * n_used <= 2048. */
 int pulsar_moe_group_csr(void *gptrs, void *starts, void *pairs, const void *ptrs,
                          uint32_t n_tok, uint32_t n_used, uint32_t max_groups);
+
+/* The CSR by expert of a chunk of any length, straight from the router's ids
+ * (pulsar_moe_group_csr takes at most 2048 pairs): group e < n_expert is bank
+ * expert e, its pairs (token << 4 | slot) in (token, slot) order, empty for an
+ * expert nothing selects; group n_expert + i is shared slot k_used + i of every
+ * token. Writes gptrs [n_expert + n_shared], starts [n_expert + n_shared + 1]
+ * and pairs [starts[n_expert + n_shared]] (room for n_tok * (k_used + n_shared);
+ * what lies behind the last pair is left as it is), for the grouped stages with
+ * n_group = n_expert + n_shared and n_used = k_used + n_shared. selected int32
+ * [n_tok][k_used]; ids outside [0, n_expert) get no pair, so the caller zeroes
+ * partial as for any CSR. slot_weights f32 [n_tok][k_used + n_shared], left out
+ * where NULL: router_weights [n_tok][k_used], then 1 for the shared slots.
+ * n_expert <= 1024, k_used + n_shared <= 16, n_shared <= 4, n_tok <= 2^28, n_tok * (k_used +
+ * n_shared) < 2^31; bank and shared are host pointers read at launch. */
+int pulsar_moe_group_ids(void *gptrs, void *starts, void *pairs, void *slot_weights,
+                         const void *selected, const void *router_weights,
+                         const pulsar_expert_bank *bank, uint32_t n_expert,
+                         const pulsar_expert_ptrs *shared, uint32_t n_shared, uint32_t n_tok,
+                         uint32_t k_used);
 
 /* pulsar_router_select (softmax_mode 0 or 1, no sink slots) +
  * pulsar_moe_route_ptrs + pulsar_moe_group_csr in one launch (no reference

@@ -50,6 +50,9 @@ SIGNATURES = {
                                _vp, _u32, _u32, _u32, _u64, _u32, _u32],
     "pulsar_moe_down_f32": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u64, _u32, _u32],
     "pulsar_moe_down_biased": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u64, _u32],
+    "pulsar_matmul_kq_fused": [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u64, _u32, _u32, _u64, _u64],
+    "pulsar_router_select_groups": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _f32, _u32],
+    "pulsar_moe_group_ids": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _u32, _u32, _u32],
     "pulsar_moe_selftest": [],
     "pulsar_router_selftest": [],
 }

@@ -5,6 +5,7 @@
 // registers for the whole kernel. Weight loads are 16-byte loads at the
 // formats' native (unaligned) offsets; consecutive lanes read consecutive
 // bytes of a row, so every wave-wide load is one contiguous span.
+#include "pk_epilogue.h"
 #include "pk_rowdot.h"
 
 // token chunks of at least this many tokens go to the MFMA kernel
@@ -17,10 +18,12 @@ namespace pk {
 // tile.hip, mmq.hip: matrix-core kernels for token chunks; -1 when one has no
 // kernel for the format or the shape (the caller then uses the next, and the
 // lane kernels last)
+template <typename E>
 int launch_tile_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
-                     uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes);
+                     uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi);
+template <typename E>
 int launch_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
-                uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes);
+                uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi);
 
 // Each wave streams row passes pass0, pass0 + n_waves, ...: the row's
 // weight units are requested first, then (once per wave) the token's
@@ -29,14 +32,14 @@ int launch_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_block
 #ifndef PK_MV_TPB
 #define PK_MV_TPB 256u
 #endif
-template <uint32_t Q, uint32_t T, uint32_t UPLMAX, uint32_t RPW, uint32_t L2>
+template <uint32_t Q, uint32_t T, uint32_t UPLMAX, uint32_t RPW, uint32_t L2, typename E>
 __global__ __launch_bounds__(PK_MV_TPB) void matvec_kernel(float *__restrict__ out,
                                                      const uint8_t *__restrict__ w,
                                                      const pulsar_block_q8_K *__restrict__ xq,
                                                      uint32_t n_units, uint32_t nblk32,
                                                      uint32_t lpr_log2, uint32_t in_blocks,
                                                      uint32_t out_dim, uint32_t n_tok,
-                                                     uint64_t row_bytes, uint32_t n_pass) {
+                                                     uint64_t row_bytes, uint32_t n_pass, E epi) {
     PK_FMT_LUT(Q)
     const RowGeom rg = row_geom<L2>(n_units, nblk32, lpr_log2);
     const uint32_t rpp = 64u >> rg.lpr_log2;
@@ -64,9 +67,11 @@ __global__ __launch_bounds__(PK_MV_TPB) void matvec_kernel(float *__restrict__ o
             const bool row_ok = row < out_dim;
 #pragma unroll
             for (uint32_t t = 0; t < T; t++) {
+                const uint32_t tok = t0 + t < n_tok ? t0 + t : n_tok - 1u;
+                const auto got = epi.get(tok, row_ok ? row : 0u);
                 float acc = row_partial<Q, UPLMAX>(row_ok, rg, wu[p], a[t], lut);
                 acc = row_finish(acc, rg);
-                if (row_ok && rg.holds_row() && t0 + t < n_tok) out[(uint64_t)(t0 + t) * out_dim + row] = acc;
+                if (row_ok && rg.holds_row() && t0 + t < n_tok) epi.put(out, out_dim, t0 + t, row, acc, got);
             }
         }
         base += n_waves * RPW;
@@ -85,11 +90,11 @@ __global__ __launch_bounds__(PK_MV_TPB) void matvec_kernel(float *__restrict__ o
 // units and activation slices are loaded, the lane's super-block values are
 // added to its running sum, and the row total is the fixed tree of the
 // lanes' sums. T tokens per launch row (grid.y covers the rest).
-template <uint32_t Q, uint32_t T>
+template <uint32_t Q, uint32_t T, typename E>
 __global__ __launch_bounds__(256) void matvec_wide_kernel(float *__restrict__ out, const uint8_t *__restrict__ w,
                                                           const pulsar_block_q8_K *__restrict__ xq, uint32_t n_units,
                                                           uint32_t nblk32, uint32_t in_blocks, uint32_t out_dim,
-                                                          uint32_t n_tok, uint64_t row_bytes) {
+                                                          uint32_t n_tok, uint64_t row_bytes, E epi) {
     PK_FMT_LUT(Q)
     const uint32_t row = blockIdx.x * 4u + threadIdx.x / 64u;
     if (row >= out_dim) return;  // whole wave
@@ -115,7 +120,7 @@ __global__ __launch_bounds__(256) void matvec_wide_kernel(float *__restrict__ ou
 #pragma unroll
     for (uint32_t t = 0; t < T; t++) {
         const float v = row_finish(acc[t], rg);
-        if (rg.holds_row() && t0 + t < n_tok) out[(uint64_t)(t0 + t) * out_dim + row] = v;
+        if (rg.holds_row() && t0 + t < n_tok) epi.put(out, out_dim, t0 + t, row, v, epi.get(t0 + t, row));
     }
 }
 
@@ -125,10 +130,10 @@ __global__ __launch_bounds__(256) void matvec_wide_kernel(float *__restrict__ ou
 #ifndef PK_MV_WAVES
 #define PK_MV_WAVES 4096u
 #endif
-template <uint32_t Q, uint32_t T, uint32_t UPLMAX, uint32_t RPW>
+template <uint32_t Q, uint32_t T, uint32_t UPLMAX, uint32_t RPW, typename E>
 static void launch_matvec(float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t n_units,
                           uint32_t nblk32, uint32_t lpr_log2, uint32_t in_blocks, uint32_t out_dim,
-                          uint32_t n_tok, uint64_t row_bytes) {
+                          uint32_t n_tok, uint64_t row_bytes, const E &epi) {
     const uint32_t rpp = 64u >> lpr_log2;
     const uint32_t n_pass = (out_dim + rpp - 1u) / rpp;
     // up to 4096 chunks one wave each; larger matrices loop over a wave
@@ -143,23 +148,24 @@ static void launch_matvec(float *out, const uint8_t *w, const pulsar_block_q8_K 
     constexpr uint32_t wpb = PK_MV_TPB / 64u;
     const dim3 grid((waves + wpb - 1u) / wpb, (n_tok + T - 1u) / T);
     if (lpr_log2 == 6)
-        hipLaunchKernelGGL((matvec_kernel<Q, T, UPLMAX, RPW, 6>), grid, dim3(PK_MV_TPB), 0, pk::stream(), out, w,
-                           xq, n_units, nblk32, lpr_log2, in_blocks, out_dim, n_tok, row_bytes, n_pass);
+        hipLaunchKernelGGL((matvec_kernel<Q, T, UPLMAX, RPW, 6, E>), grid, dim3(PK_MV_TPB), 0, pk::stream(), out, w,
+                           xq, n_units, nblk32, lpr_log2, in_blocks, out_dim, n_tok, row_bytes, n_pass, epi);
     else
-        hipLaunchKernelGGL((matvec_kernel<Q, T, UPLMAX, RPW, 0>), grid, dim3(PK_MV_TPB), 0, pk::stream(), out, w,
-                           xq, n_units, nblk32, lpr_log2, in_blocks, out_dim, n_tok, row_bytes, n_pass);
+        hipLaunchKernelGGL((matvec_kernel<Q, T, UPLMAX, RPW, 0, E>), grid, dim3(PK_MV_TPB), 0, pk::stream(), out, w,
+                           xq, n_units, nblk32, lpr_log2, in_blocks, out_dim, n_tok, row_bytes, n_pass, epi);
 }
 
 
-template <uint32_t Q>
+template <uint32_t Q, typename E>
 static int dispatch_matvec(float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
-                           uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes) {
+                           uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi) {
     const uint32_t n_units = units_per_row(Q, in_dim);
     const uint32_t l2 = lpr_log2_for(n_units);
     const uint32_t upl = (n_units + (1u << l2) - 1u) >> l2;
     const uint32_t in_blocks = (in_dim + 255u) / 256u;
     const uint32_t nblk32 = (in_dim + 31u) / 32u;
-#define PK_MV(T, U, R) launch_matvec<Q, T, U, R>(out, w, xq, n_units, nblk32, l2, in_blocks, out_dim, n_tok, row_bytes)
+#define PK_MV(T, U, R) \
+    launch_matvec<Q, T, U, R>(out, w, xq, n_units, nblk32, l2, in_blocks, out_dim, n_tok, row_bytes, epi)
     if (upl <= 1u) {
         if (n_tok == 1u)
             PK_MV(1, 1, PK_MV_RPW);
@@ -180,14 +186,64 @@ static int dispatch_matvec(float *out, const uint8_t *w, const pulsar_block_q8_K
         // wider rows: one wave per row, streamed in 16-super-block slices
         const dim3 grid((out_dim + 3u) / 4u, n_tok <= 1u ? 1u : (n_tok + 3u) / 4u);
         if (n_tok == 1u)
-            hipLaunchKernelGGL((matvec_wide_kernel<Q, 1>), grid, dim3(256), 0, pk::stream(), out, w, xq, n_units,
-                               nblk32, in_blocks, out_dim, n_tok, row_bytes);
+            hipLaunchKernelGGL((matvec_wide_kernel<Q, 1, E>), grid, dim3(256), 0, pk::stream(), out, w, xq, n_units,
+                               nblk32, in_blocks, out_dim, n_tok, row_bytes, epi);
         else
-            hipLaunchKernelGGL((matvec_wide_kernel<Q, 4>), grid, dim3(256), 0, pk::stream(), out, w, xq, n_units,
-                               nblk32, in_blocks, out_dim, n_tok, row_bytes);
+            hipLaunchKernelGGL((matvec_wide_kernel<Q, 4, E>), grid, dim3(256), 0, pk::stream(), out, w, xq, n_units,
+                               nblk32, in_blocks, out_dim, n_tok, row_bytes, epi);
     }
 #undef PK_MV
     return launch_ok("matmul_kq launch");
+}
+
+template <typename E>
+static int dense_product(const char *what, void *out, const void *w, const void *xq, uint32_t in_dim, uint32_t out_dim,
+                         uint32_t n_tok, uint64_t row_bytes, uint32_t quant, const E &epi) {
+    float *o = (float *)out;
+    const uint8_t *wb = (const uint8_t *)w;
+    const pulsar_block_q8_K *x = (const pulsar_block_q8_K *)xq;
+    if (n_tok >= PK_MMQ_MIN_TOK) {
+        int r = launch_tile_gemm(quant, o, wb, x, in_dim, out_dim, n_tok, row_bytes, epi);
+        if (r < 0) r = launch_gemm(quant, o, wb, x, in_dim, out_dim, n_tok, row_bytes, epi);
+        if (r >= 0) return r;
+    }
+    // the dense formats of pulsar_kernels.cu:5090-5142
+#define PK_MVQ(Q) \
+    case Q: return dispatch_matvec<Q>(o, wb, x, in_dim, out_dim, n_tok, row_bytes, epi);
+    switch (quant) {
+    PK_MVQ(PULSAR_QUANT_Q4_K)
+    PK_MVQ(PULSAR_QUANT_Q6_K)
+    PK_MVQ(PULSAR_QUANT_Q2_K)
+    PK_MVQ(PULSAR_QUANT_IQ2_XXS)
+    PK_MVQ(PULSAR_QUANT_Q5_K)
+    PK_MVQ(PULSAR_QUANT_Q3_K)
+    PK_MVQ(PULSAR_QUANT_IQ4_XS)
+    PK_MVQ(PULSAR_QUANT_IQ4_NL)
+    PK_MVQ(PULSAR_QUANT_NVFP4)
+    default: return reject(what);
+    }
+#undef PK_MVQ
+}
+
+// Bytes [a, a + an) and [b, b + bn) share one
+typedef unsigned __int128 u128;
+static bool overlap(const void *a, u128 an, const void *b, u128 bn) {
+    return (u128)(uintptr_t)a < (uintptr_t)b + bn && (u128)(uintptr_t)b < (uintptr_t)a + an;
+}
+
+// Whether the rows of out may be written while those of residual are read:
+// the same rows (an element is read before it is written), apart, or columns
+// of one wider array that share no float.
+static bool rows_allow(const void *out, uint64_t out_stride, const void *res, uint64_t res_stride, uint32_t dim,
+                       uint32_t n_tok) {
+    if (out == res && out_stride == res_stride) return true;
+    auto bytes = [&](uint64_t stride) { return 4 * ((u128)(n_tok - 1u) * stride + dim); };
+    if (!overlap(out, bytes(out_stride), res, bytes(res_stride))) return true;
+    if (out_stride != res_stride) return false;
+    const u128 row = 4 * (u128)out_stride, width = 4 * (u128)dim;
+    const uint64_t a = (uint64_t)(uintptr_t)out, b = (uint64_t)(uintptr_t)res;
+    const u128 apart = b >= a ? (b - a) % row : (row - (a - b) % row) % row;
+    return apart >= width && apart + width <= row;
 }
 
 }  // namespace pk
@@ -203,28 +259,29 @@ extern "C" int pulsar_matmul_kq(void *out, const void *w, const void *xq, uint32
     if (!out || !w || !xq || in_dim == 0 || in_dim % 256u != 0 || out_dim == 0 || n_tok == 0 ||
         row_bytes == 0)
         return pk::reject("matmul_kq");
-    float *o = (float *)out;
-    const uint8_t *wb = (const uint8_t *)w;
-    const pulsar_block_q8_K *x = (const pulsar_block_q8_K *)xq;
-    if (n_tok >= PK_MMQ_MIN_TOK) {
-        int r = pk::launch_tile_gemm(quant, o, wb, x, in_dim, out_dim, n_tok, row_bytes);
-        if (r < 0) r = pk::launch_gemm(quant, o, wb, x, in_dim, out_dim, n_tok, row_bytes);
-        if (r >= 0) return r;
-    }
-    // the dense formats of pulsar_kernels.cu:5090-5142
-#define PK_MVQ(Q) \
-    case Q: return pk::dispatch_matvec<Q>(o, wb, x, in_dim, out_dim, n_tok, row_bytes);
-    switch (quant) {
-    PK_MVQ(PULSAR_QUANT_Q4_K)
-    PK_MVQ(PULSAR_QUANT_Q6_K)
-    PK_MVQ(PULSAR_QUANT_Q2_K)
-    PK_MVQ(PULSAR_QUANT_IQ2_XXS)
-    PK_MVQ(PULSAR_QUANT_Q5_K)
-    PK_MVQ(PULSAR_QUANT_Q3_K)
-    PK_MVQ(PULSAR_QUANT_IQ4_XS)
-    PK_MVQ(PULSAR_QUANT_IQ4_NL)
-    PK_MVQ(PULSAR_QUANT_NVFP4)
-    default: return pk::reject("matmul_kq (quant)");
-    }
-#undef PK_MVQ
+    return pk::dense_product("matmul_kq (quant)", out, w, xq, in_dim, out_dim, n_tok, row_bytes, quant,
+                             pk::PlainOut{});
+}
+
+extern "C" int pulsar_matmul_kq_fused(void *out, const void *w, const void *xq, const void *bias,
+                                      const void *residual, uint32_t in_dim, uint32_t out_dim, uint32_t n_tok,
+                                      uint64_t row_bytes, uint32_t quant, uint32_t act, uint64_t out_stride,
+                                      uint64_t res_stride) {
+    quant &= ~PULSAR_QUANT_A4_OK;
+    if (out_stride == 0) out_stride = out_dim;
+    if (res_stride == 0) res_stride = out_dim;
+    if (!out || !w || !xq || in_dim == 0 || in_dim % 256u != 0 || out_dim == 0 || n_tok == 0 || row_bytes == 0 ||
+        act > PULSAR_EPI_SIGMOID || out_stride < out_dim || (residual && res_stride < out_dim))
+        return pk::reject("matmul_kq_fused");
+    const pk::u128 out_bytes = 4 * ((pk::u128)(n_tok - 1u) * out_stride + out_dim);
+    const pk::u128 xq_bytes = (pk::u128)n_tok * (in_dim / 256u) * 292u;
+    if (out_bytes >> 62 || (residual && !pk::rows_allow(out, out_stride, residual, res_stride, out_dim, n_tok)) ||
+        pk::overlap(out, out_bytes, xq, xq_bytes) || pk::overlap(out, out_bytes, w, (pk::u128)out_dim * row_bytes) ||
+        (bias && pk::overlap(out, out_bytes, bias, 4 * (pk::u128)out_dim)))
+        return pk::reject("matmul_kq_fused (overlap)");
+    // what is left out is read from xq, which has at least a q8_K block
+    const pk::FusedOut epi = {bias ? (const float *)bias : (const float *)xq,
+                              residual ? (const float *)residual : (const float *)xq, out_stride, res_stride, act,
+                              bias ? 1u : 0u, residual ? 1u : 0u};
+    return pk::dense_product("matmul_kq_fused (quant)", out, w, xq, in_dim, out_dim, n_tok, row_bytes, quant, epi);
 }

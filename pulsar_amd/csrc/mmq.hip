@@ -22,6 +22,7 @@
 // ones, and every sum is over whole lane groups.
 #include <type_traits>
 
+#include "pk_epilogue.h"
 #include "pk_rowdot.h"
 #include "pk_route.h"
 
@@ -197,10 +198,11 @@ PK_DEV uint32_t pair_sum_bytes(uint4 b, bool high) {
 // the D - 1 chunks behind the one needed; only the last group's requests
 // past the end of K (clamped to its last super-block) are wasted.
 // The C partials of a row tile are added in wave order (deterministic).
-template <uint32_t Q, uint32_t RT, uint32_t C, uint32_t NT, uint32_t D>
+template <uint32_t Q, uint32_t RT, uint32_t C, uint32_t NT, uint32_t D, typename E>
 __global__ __launch_bounds__(64 * RT * C) void mmq_gemm_kernel(float *__restrict__ out, const uint8_t *__restrict__ w,
                                                                const pulsar_block_q8_K *__restrict__ xq, uint32_t nb,
-                                                               uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes) {
+                                                               uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes,
+                                                               E epi) {
     using F = GemmFmt<Q>;
     constexpr uint32_t NW = RT * C, NTH = 64u * NW, TOK = 16u * NT, ROWS = 16u * RT;
     constexpr uint32_t kSlot = 16u * F::kChunks;
@@ -483,11 +485,12 @@ __global__ __launch_bounds__(64 * RT * C) void mmq_gemm_kernel(float *__restrict
     for (uint32_t e = tid; e < TOK * ROWS; e += NTH) {
         const uint32_t row = e % ROWS, tok = e / ROWS;
         if (r0 + row < out_dim && t0 + tok < n_tok) {
+            const auto got = epi.get(t0 + tok, r0 + row);
             const uint32_t prt = row / 16u;
             float v = part[((prt * C) * 16u + row % 16u) * (TOK + 1u) + tok];
 #pragma unroll
             for (uint32_t k = 1; k < C; k++) v += part[((prt * C + k) * 16u + row % 16u) * (TOK + 1u) + tok];
-            out[(uint64_t)(t0 + tok) * out_dim + r0 + row] = v;
+            epi.put(out, out_dim, t0 + tok, r0 + row, v, got);
         }
     }
 }
@@ -512,13 +515,13 @@ __global__ __launch_bounds__(64 * RT * C) void mmq_gemm_kernel(float *__restrict
 #define PK_GEMM_D_R32 2u
 #endif
 
-template <uint32_t Q>
+template <uint32_t Q, typename E>
 static int launch_gemm_q(float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t nb, uint32_t out_dim,
-                         uint32_t n_tok, uint64_t row_bytes) {
+                         uint32_t n_tok, uint64_t row_bytes, const E &epi) {
 #define PK_GEMM(RT, C, NT, D)                                                                                \
-    hipLaunchKernelGGL((mmq_gemm_kernel<Q, RT, C, NT, D>), dim3((n_tok + 16u * NT - 1u) / (16u * NT),         \
+    hipLaunchKernelGGL((mmq_gemm_kernel<Q, RT, C, NT, D, E>), dim3((n_tok + 16u * NT - 1u) / (16u * NT),         \
                                                                 (out_dim + 16u * RT - 1u) / (16u * RT)),       \
-                       dim3(64 * RT * C), 0, pk::stream(), out, w, xq, nb, out_dim, n_tok, row_bytes)
+                       dim3(64 * RT * C), 0, pk::stream(), out, w, xq, nb, out_dim, n_tok, row_bytes, epi)
     // below 8192 rows a 32-row tile leaves CUs idle (4096 rows: 128 blocks);
     // 16-row tiles with 8 super-blocks per chunk measured fastest there
     // (Q4_K 4096 x 4096, 16 tokens: 8.7 -> 6.9 us), 32-row tiles with 4
@@ -543,18 +546,23 @@ static int launch_gemm_q(float *out, const uint8_t *w, const pulsar_block_q8_K *
 // MFMA GEMM for token chunks / prefill (the reference's prefill GEMM formats,
 // pulsar_kernels.cu:4914-4916: Q4_K, Q6_K, NVFP4, plus Q5_K, which the
 // reference runs through its per-token matvec); -1 for other formats.
+template <typename E>
 int launch_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
-                uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes) {
+                uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi) {
     const uint32_t nb = in_dim / 256u;
     if ((uint64_t)((out_dim + 31u) / 32u) > 65535u) return -1;  // grid y
     switch (quant) {
-    case PULSAR_QUANT_Q6_K: return launch_gemm_q<PULSAR_QUANT_Q6_K>(out, w, xq, nb, out_dim, n_tok, row_bytes);
-    case PULSAR_QUANT_Q4_K: return launch_gemm_q<PULSAR_QUANT_Q4_K>(out, w, xq, nb, out_dim, n_tok, row_bytes);
-    case PULSAR_QUANT_NVFP4: return launch_gemm_q<PULSAR_QUANT_NVFP4>(out, w, xq, nb, out_dim, n_tok, row_bytes);
-    case PULSAR_QUANT_Q5_K: return launch_gemm_q<PULSAR_QUANT_Q5_K>(out, w, xq, nb, out_dim, n_tok, row_bytes);
+    case PULSAR_QUANT_Q6_K: return launch_gemm_q<PULSAR_QUANT_Q6_K>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi);
+    case PULSAR_QUANT_Q4_K: return launch_gemm_q<PULSAR_QUANT_Q4_K>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi);
+    case PULSAR_QUANT_NVFP4: return launch_gemm_q<PULSAR_QUANT_NVFP4>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi);
+    case PULSAR_QUANT_Q5_K: return launch_gemm_q<PULSAR_QUANT_Q5_K>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi);
     default: return -1;
     }
 }
+template int launch_gemm(uint32_t, float *, const uint8_t *, const pulsar_block_q8_K *, uint32_t, uint32_t, uint32_t,
+                         uint64_t, const PlainOut &);
+template int launch_gemm(uint32_t, float *, const uint8_t *, const pulsar_block_q8_K *, uint32_t, uint32_t, uint32_t,
+                         uint64_t, const FusedOut &);
 
 // ------------------------------------ grouped Q2_K / IQ2_XXS / MXFP4 (MoE) --
 // Block = 16 rows per wave (kGqWaves waves: 64 rows, MXFP4 192) x up to

@@ -8,6 +8,7 @@
 //     cores 34%; its 256 registers leave two waves per SIMD, which overlap
 //     these only in part: 30% of a wave's time waits for LDS and memory, 30%
 //     for an issue slot.
+#include "pk_epilogue.h"
 #include "pk_tile.h"
 
 namespace pk {
@@ -16,11 +17,11 @@ namespace pk {
 // robin, each with its own L2: XCD x takes the x-th eighth of the (row block,
 // token tile) items, token tiles fastest, so a row block's weights are read
 // by one XCD.
-template <uint32_t Q, uint32_t WR, uint32_t WK, uint32_t NS>
+template <uint32_t Q, uint32_t WR, uint32_t WK, uint32_t NS, typename E>
 __global__ __launch_bounds__(256, 2) void tile_gemm_kernel(float *__restrict__ out, const uint8_t *__restrict__ w,
                                                            const pulsar_block_q8_K *__restrict__ xq, uint32_t nb,
                                                            uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes,
-                                                           uint32_t n_tt, uint32_t n_item) {
+                                                           uint32_t n_tt, uint32_t n_item, E epi) {
     using T = Tile<Q, WR, WK, NS>;
     __shared__ __align__(16) uint8_t buf0[T::kBuf];
     __shared__ __align__(16) uint8_t buf1[T::kBuf];
@@ -41,9 +42,10 @@ __global__ __launch_bounds__(256, 2) void tile_gemm_kernel(float *__restrict__ o
         for (uint32_t r = 0; r < 4; r++) {
             const uint32_t t = 16u * n + 4u * q + r;
             if (!T::mine(n, r, wave / WR) || t >= np) continue;
-            float *o = out + (uint64_t)(t0 + t) * out_dim + row;
-            if (row < out_dim) o[0] = tile.acc[n][0][r];
-            if (row + 16u < out_dim) o[16] = tile.acc[n][1][r];
+            const auto got0 = epi.get(t0 + t, row < out_dim ? row : out_dim - 1u);
+            const auto got1 = epi.get(t0 + t, row + 16u < out_dim ? row + 16u : out_dim - 1u);
+            if (row < out_dim) epi.put(out, out_dim, t0 + t, row, tile.acc[n][0][r], got0);
+            if (row + 16u < out_dim) epi.put(out, out_dim, t0 + t, row + 16u, tile.acc[n][1][r], got1);
         }
 }
 
@@ -52,17 +54,17 @@ static uint64_t tile_items(uint32_t out_dim, uint32_t n_tok) {
     return (uint64_t)((n_tok + 16u * NS - 1u) / (16u * NS)) * ((out_dim + 32u * WR - 1u) / (32u * WR));
 }
 
-template <uint32_t Q>
+template <uint32_t Q, typename E>
 static int launch_tile_gemm_q(float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t nb,
-                              uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes) {
+                              uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi) {
 #define PK_TILE_FITS(WR, WK, NS) (tile_items<Q, WR, WK, NS>(out_dim, n_tok) <= kTileSlots)
 #define PK_TILE(WR, WK, NS)                                                                                        \
     do {                                                                                                           \
         const uint64_t n_item = tile_items<Q, WR, WK, NS>(out_dim, n_tok);                                         \
         if (n_item > 0x7ffffff0ull) return -1;                                                                     \
-        hipLaunchKernelGGL((tile_gemm_kernel<Q, WR, WK, NS>), dim3((uint32_t)((n_item + 7u) & ~7ull)), dim3(256), 0, \
+        hipLaunchKernelGGL((tile_gemm_kernel<Q, WR, WK, NS, E>), dim3((uint32_t)((n_item + 7u) & ~7ull)), dim3(256), 0, \
                            pk::stream(), out, w, xq, nb, out_dim, n_tok, row_bytes,                                 \
-                           (n_tok + 16u * NS - 1u) / (16u * NS), (uint32_t)n_item);                                 \
+                           (n_tok + 16u * NS - 1u) / (16u * NS), (uint32_t)n_item, epi);                            \
     } while (0)
     // The finest tile whose blocks are all in flight at once, else the widest:
     // a block's time falls with its rows and tokens (fewer steps with K split),
@@ -85,8 +87,9 @@ static int launch_tile_gemm_q(float *out, const uint8_t *w, const pulsar_block_q
 }
 
 // -1: no tile kernel for the format or the shape
+template <typename E>
 int launch_tile_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
-                     uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes) {
+                     uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi) {
     const uint32_t nb = in_dim / 256u;
     if (nb > 65536u) return -1;  // a tile's activation offsets are 32 bits
     // the tile's copies to LDS move whole dwords of xq, the other kernels load
@@ -138,7 +141,7 @@ int launch_tile_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_
         if (rows4 < least || (nb < 4u && rows4 * nb < least_nb)) return -1;
     }
 #define PK_TG(Q) \
-    case Q: return launch_tile_gemm_q<Q>(out, w, xq, nb, out_dim, n_tok, row_bytes);
+    case Q: return launch_tile_gemm_q<Q>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi);
     switch (quant) {
         PK_TG(PULSAR_QUANT_Q4_K)
         PK_TG(PULSAR_QUANT_Q5_K)
@@ -151,5 +154,9 @@ int launch_tile_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_
     }
 #undef PK_TG
 }
+template int launch_tile_gemm(uint32_t, float *, const uint8_t *, const pulsar_block_q8_K *, uint32_t, uint32_t,
+                              uint32_t, uint64_t, const PlainOut &);
+template int launch_tile_gemm(uint32_t, float *, const uint8_t *, const pulsar_block_q8_K *, uint32_t, uint32_t,
+                              uint32_t, uint64_t, const FusedOut &);
 
 }  // namespace pk

@@ -29,6 +29,11 @@ QUANT_A4_OK = 0x8000_0000
 ACT_SILU = 0
 ACT_SWIGLU_OAI = 2
 
+# epilogue of the dense product (PULSAR_EPI_*) and scores of the routing with
+# expert groups (PULSAR_SCORE_*) in include/pulsar_moe.h
+EPI_NONE, EPI_SILU, EPI_GELU, EPI_RELU, EPI_SIGMOID = range(5)
+SCORE_SIGMOID, SCORE_SOFTMAX = range(2)
+
 QK_K = 256
 Q8_K_BLOCK_BYTES = 292  # f32 d, i8 qs[256], i16 bsums[16]
 EXPERT_PTRS_BYTES = 48  # six pointers

@@ -55,6 +55,61 @@ def matmul_kq(out, w, xq, in_dim: int, out_dim: int, n_tok: int, row_bytes: int,
     )
 
 
+def _room(buf, nbytes: int, op: str, what: str) -> int:
+    """The device address of `buf`, which the launch uses the first nbytes
+    bytes of; a tensor has to be contiguous, that large and on the current
+    device (a raw address is the caller's word for all three)."""
+    if buf is None or isinstance(buf, int) or not hasattr(buf, "data_ptr"):
+        return _ptr(buf)
+    at = _ptr(buf)
+    if not buf.is_contiguous() or buf.numel() * buf.element_size() < nbytes:
+        raise ValueError(f"{op}: {what} has to be contiguous and hold {nbytes} bytes")
+    _same_device(buf, op, what)
+    return at
+
+
+def _same_device(buf, op: str, what: str) -> None:
+    if buf.get_device() != _lib.torch.cuda.current_device():
+        raise ValueError(f"{op}: {what} is not on the current device")
+
+
+def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str) -> int:
+    """The device address of n_rows rows of dim floats, `stride` floats apart.
+    A tensor may be a view of columns of a wider array: it has to be f32 [..,
+    dim] with that stride, or contiguous and large enough."""
+    if buf is None or isinstance(buf, int) or not hasattr(buf, "data_ptr"):
+        return _ptr(buf)
+    at = _ptr(buf)
+    if buf.element_size() != 4:
+        raise ValueError(f"{op}: {what} has to be f32")
+    if buf.is_contiguous():
+        ok = buf.numel() >= (n_rows - 1) * stride + dim
+    else:
+        ok = (buf.dim() == 2 and buf.shape[0] >= n_rows and buf.shape[1] >= dim and buf.stride(1) == 1
+              and buf.stride(0) == stride)
+    if not ok:
+        raise ValueError(f"{op}: {what} has to hold {n_rows} rows of {dim} f32 values {stride} apart")
+    _same_device(buf, op, what)
+    return at
+
+
+def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok: int, row_bytes: int, quant: int,
+                    act: int = 0, out_stride: int = 0, res_stride: int = 0) -> None:
+    """matmul_kq with its epilogue in the same launch: out[t] = act(W x_t +
+    bias) + residual[t] (formats.EPI_* codes; bias and residual may be None).
+    Strides in floats, 0 for packed rows; residual may be out itself."""
+    op = "matmul_kq_fused"
+    xq_bytes, so, sr = n_tok * -(-in_dim // 256) * 292, out_stride or out_dim, res_stride or out_dim
+    _check(
+        _lib.load().pulsar_matmul_kq_fused(
+            _rows(out, n_tok, out_dim, so, op, "out"), _room(w, (out_dim - 1) * row_bytes, op, "w"),
+            _room(xq, xq_bytes, op, "xq"), _room(bias, 4 * out_dim, op, "bias"),
+            _rows(residual, n_tok, out_dim, sr, op, "residual"), in_dim, out_dim, n_tok, row_bytes, quant, act,
+            out_stride, res_stride),
+        op,
+    )
+
+
 def moe_pair_swiglu(mid, ptrs, weights, x, in_dim: int, mid_dim: int, n_used: int, n_tok: int,
                     row_bytes: int, quant: int, act_op: int) -> None:
     _check(
@@ -124,6 +179,21 @@ def router_select(selected, weights, logits, bias, n_expert: int, k_used: int, w
     )
 
 
+def router_select_groups(selected, weights, logits, bias, n_expert: int, k_used: int, n_group: int, topk_group: int,
+                         group_top: int, score: int, renorm: bool, weight_scale: float, n_tok: int) -> None:
+    """Top-k of the experts of the topk_group best of n_group expert groups
+    (a group's score: its group_top largest score + bias; formats.SCORE_*),
+    the weights the winners' scores, renormalised if renorm, times weight_scale."""
+    op = "router_select_groups"
+    _check(
+        _lib.load().pulsar_router_select_groups(
+            _room(selected, 4 * n_tok * k_used, op, "selected"), _room(weights, 4 * n_tok * k_used, op, "weights"),
+            _room(logits, 4 * n_tok * n_expert, op, "logits"), _room(bias, 4 * n_expert, op, "bias"), n_expert, k_used,
+            n_group, topk_group, group_top, score, int(bool(renorm)), weight_scale, n_tok),
+        op,
+    )
+
+
 def matmul_f32(out, w, x, in_dim: int, out_dim: int, n_tok: int) -> None:
     _check(_lib.load().pulsar_matmul_f32(_ptr(out), _ptr(w), _ptr(x), in_dim, out_dim, n_tok), "matmul_f32")
 
@@ -168,6 +238,26 @@ def moe_group_csr(gptrs, starts, pairs, ptrs, n_tok: int, n_used: int, max_group
         _lib.load().pulsar_moe_group_csr(_ptr(gptrs), _ptr(starts), _ptr(pairs), _ptr(ptrs), n_tok, n_used,
                                          max_groups),
         "moe_group_csr",
+    )
+
+
+def moe_group_ids(gptrs, starts, pairs, slot_weights, selected, router_weights, bank: ExpertBank, n_expert: int,
+                  shared, n_tok: int, k_used: int) -> None:
+    """The CSR by expert of a chunk of any length from the router's ids: group e
+    is bank expert e, then one group per shared slot; the grouped stages take it
+    with n_group = n_expert + len(shared). slot_weights (None: left out) gets
+    router_weights and the shared slots' ones."""
+    op = "moe_group_ids"
+    arr, n_shared = _shared_array(shared)
+    groups, slots = n_expert + n_shared, k_used + n_shared
+    _check(
+        _lib.load().pulsar_moe_group_ids(
+            _room(gptrs, EXPERT_PTRS_BYTES * groups, op, "gptrs"), _room(starts, 4 * (groups + 1), op, "starts"),
+            _room(pairs, 4 * n_tok * slots, op, "pairs"), _room(slot_weights, 4 * n_tok * slots, op, "slot_weights"),
+            _room(selected, 4 * n_tok * k_used, op, "selected"),
+            _room(router_weights, 4 * n_tok * k_used, op, "router_weights"), ctypes.byref(bank), n_expert,
+            ctypes.cast(arr, ctypes.c_void_p), n_shared, n_tok, k_used),
+        op,
     )
 
 
