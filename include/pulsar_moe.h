@@ -231,8 +231,8 @@ int pulsar_router_select(void *selected, void *weights, const void *logits,
  *     falling order, ties to the lower id, each expert once; -1 with weight 0
  *     where fewer than k_used are left
  *   weights f32 [n_tok][k_used]: the winners' s (without the bias); renorm != 0:
- *     over their sum (sigmoid: at least 2^-14, as pulsar_router_select); times
- *     weight_scale
+ *     over their sum (sigmoid: at least 2^-14, as pulsar_router_select; softmax:
+ *     all 0 where every winner's s is 0 in 64 bits); times weight_scale
  * Ids are decided as c stands in 64 bits, whatever f32 would round it to.
  * n_expert <= 1024, a multiple of n_group <= 64; k_used <= 64 and <= the
  * experts of topk_group groups. */

@@ -2,17 +2,16 @@
 // ids (pulsar_moe_group_ids).
 //
 // A block per group. Block e scans every id: those below e (and not negative)
-// count into the group's start, a ballot marks those equal to e, and the marks,
-// in order, are the group's pairs. No workspace, no atomics, one launch, and the
-// pairs of a group come out in (token, slot) order. The blocks read the same
-// ids, from L2: n ids cost each block n / 16 wave loads.
+// count into the group's start, a ballot per 64 ids marks those equal to e, and
+// the marks, in order, are the group's pairs. No workspace, no atomics, one
+// launch, and the pairs of a group come out in (token, slot) order. The blocks
+// read the same ids, from L2; a mark stays in the registers of one lane (ballot
+// i of a wave in lane i % 64), so that the lanes unpack them side by side.
 #include "pk_route.h"
 
 namespace pk {
 
 constexpr uint32_t kGidThreads = 1024, kGidWaves = kGidThreads / 64u;
-constexpr uint32_t kGidMarked = 1u << 18;  // ids whose marks fit 32 KiB of LDS
-
 struct GroupIds {
     pulsar_expert_ptrs *gptrs;
     uint32_t *starts, *pairs;
@@ -21,13 +20,15 @@ struct GroupIds {
     const float *router_w;
     pulsar_expert_bank bank;
     SharedSlots shared;
-    uint32_t n_expert, n_shared, n_tok, k_used;
+    uint32_t n_expert, n_shared, n_tok, k_used, kept;
 };
 
 // Blocks [0, n_expert + n_shared): the groups; the blocks after them copy the
 // router's weights next to the shared slots' ones.
+// R: 64-bit marks a lane keeps, for up to 65536 R ids; where there are more,
+// a.kept is 0 and the blocks read the ids twice.
+template <uint32_t R>
 __global__ __launch_bounds__(kGidThreads) void group_ids_kernel(GroupIds a) {
-    extern __shared__ uint64_t mark[];  // 4 ballots per 256 ids
     __shared__ uint32_t below_l[kGidWaves], equal_l[kGidWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t g = blockIdx.x, n = a.n_tok * a.k_used, n_group = a.n_expert + a.n_shared;
@@ -41,35 +42,53 @@ __global__ __launch_bounds__(kGidThreads) void group_ids_kernel(GroupIds a) {
         return;
     }
     const uint32_t e = g < a.n_expert ? g : a.n_expert;
-    // wave w takes the 256-id pieces [w per, (w + 1) per)
-    const uint32_t pieces = (n + 255u) / 256u, per = (pieces + kGidWaves - 1u) / kGidWaves;
-    const uint32_t p0 = wave * per, p1 = p0 + per < pieces ? p0 + per : pieces;
-    const bool marked = n <= kGidMarked;
-    // the ids of a piece: lane l those at 4 l .. 4 l + 3; past the end -1, which is no expert
-    auto ids_of = [&](uint32_t p, int32_t (&id)[4]) {
-        const uint32_t at = p * 256u + 4u * lane;
-        if (p * 256u + 256u <= n) {
-            const uint4 v = ld128((const uint8_t *)(a.sel + at));
-            id[0] = (int32_t)v.x, id[1] = (int32_t)v.y, id[2] = (int32_t)v.z, id[3] = (int32_t)v.w;
+    // wave w takes the 64-id strips [w per, (w + 1) per), eight at a time
+    const uint32_t strips = (n + 63u) / 64u, per = (strips + kGidWaves - 1u) / kGidWaves;
+    const uint32_t p0 = wave * per < strips ? wave * per : strips, p1 = p0 + per < strips ? p0 + per : strips;
+    constexpr uint32_t U = 8;
+    auto ids_of = [&](uint32_t p, int32_t (&id)[U]) {
+        if ((p + U) * 64u <= n) {
+            const int32_t *at = a.sel + (uint64_t)p * 64u + lane;
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) id[u] = at[64u * u];
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) id[j] = at + j < n ? a.sel[at + j] : -1;
+            for (uint32_t u = 0; u < U; u++) {
+                const uint64_t i = (uint64_t)(p + u) * 64u + lane;
+                const int32_t v = a.sel[i < n ? i : n - 1u];
+                id[u] = i < n ? v : -1;  // no expert
+            }
         }
     };
-    uint32_t below = 0, equal = 0;
-    for (uint32_t p = p0; p < p1; p++) {
-        int32_t id[4];
-        ids_of(p, id);
-        uint64_t m[4];
+    uint64_t mark[R];
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            below += (uint32_t)id[j] < e ? 1u : 0u;
-            m[j] = __ballot(g < a.n_expert && id[j] == (int32_t)e);
-            equal += (uint32_t)__builtin_popcountll(m[j]);
+    for (uint32_t q = 0; q < R; q++) mark[q] = 0ull;
+    // the marks of strips p .. of one register, strips past p1 none
+    auto marks_of = [&](uint32_t p, uint32_t &below, uint32_t &equal) {
+        uint64_t mk = 0ull;
+        const uint32_t end = p + 64u < p1 ? p + 64u : p1;
+        for (uint32_t q = p; q < end; q += U) {
+            int32_t id[U];
+            ids_of(q, id);
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {
+                if (q + u >= end) break;  // uniform
+                below += (uint32_t)__builtin_popcountll(__ballot((uint32_t)id[u] < e));
+                const uint64_t eq = __ballot(id[u] == (int32_t)e);
+                equal += (uint32_t)__builtin_popcountll(eq);
+                mk = lane == q + u - p ? eq : mk;
+            }
         }
-        if (marked && lane < 4u) mark[4u * p + lane] = lane == 0u ? m[0] : lane == 1u ? m[1] : lane == 2u ? m[2] : m[3];
+        return mk;
+    };
+    uint32_t below = 0, equal = 0;
+    if (a.kept) {
+#pragma unroll
+        for (uint32_t q = 0; q < R; q++)
+            if (p0 + 64u * q < p1) mark[q] = marks_of(p0 + 64u * q, below, equal);
+    } else {
+        for (uint32_t p = p0; p < p1; p += 64u) marks_of(p, below, equal);
     }
-    below = (uint32_t)group_sum<64>((int32_t)below);
     if (lane == 0) {
         below_l[wave] = below;
         equal_l[wave] = equal;
@@ -89,29 +108,33 @@ __global__ __launch_bounds__(kGidThreads) void group_ids_kernel(GroupIds a) {
         count = a.n_tok;
     } else {
         at += start;
-        for (uint32_t p = p0; p < p1; p++) {
-            uint64_t m[4];
-            if (marked) {
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) m[j] = mark[4u * p + j];
-            } else {
-                int32_t id[4];
-                ids_of(p, id);
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) m[j] = __ballot(id[j] == (int32_t)e);
+        // each lane the pairs of its mark, behind those of the lanes below it
+        auto unpack = [&](uint32_t p, uint64_t mk) {
+            const uint32_t own = (uint32_t)__builtin_popcountll(mk);
+            int32_t x = (int32_t)own;  // inclusive scan over the wave
+            x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
+            x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+            x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+            x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+            x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+            x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+            uint32_t q = at + (uint32_t)x - own;
+            const uint32_t i0 = (p + lane) * 64u;
+            while (mk) {
+                const uint32_t i = i0 + (uint32_t)__builtin_ctzll(mk), t = i / a.k_used;
+                a.pairs[q++] = (t << 4) | (i - t * a.k_used);
+                mk &= mk - 1ull;
             }
-            if ((m[0] | m[1] | m[2] | m[3]) == 0ull) continue;
-            const uint64_t lower = (1ull << lane) - 1ull;
-            uint32_t q = at;
+            at += (uint32_t)__builtin_amdgcn_readlane(x, 63);
+        };
+        if (a.kept) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) q += (uint32_t)__builtin_popcountll(m[j] & lower);
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                if (m[j] >> lane & 1u) {
-                    const uint32_t i = p * 256u + 4u * lane + j, t = i / a.k_used;
-                    a.pairs[q++] = (t << 4) | (i - t * a.k_used);
-                }
-                at += (uint32_t)__builtin_popcountll(m[j]);
+            for (uint32_t q = 0; q < R; q++)
+                if (p0 + 64u * q < p1) unpack(p0 + 64u * q, mark[q]);
+        } else {
+            for (uint32_t p = p0; p < p1; p += 64u) {
+                uint32_t b = 0, c = 0;
+                unpack(p, marks_of(p, b, c));
             }
         }
     }
@@ -135,11 +158,16 @@ extern "C" int pulsar_moe_group_ids(void *gptrs, void *starts, void *pairs, void
         return pk::reject("moe group ids");
     pk::GroupIds a = {(pulsar_expert_ptrs *)gptrs, (uint32_t *)starts, (uint32_t *)pairs, (float *)slot_weights,
                       (const int32_t *)selected, (const float *)router_weights, *bank, {}, n_expert, n_shared, n_tok,
-                      k_used};
+                      k_used, 1u};
     for (uint32_t i = 0; i < n_shared; i++) a.shared.p[i] = shared[i];
-    const uint32_t n = n_tok * k_used, copies = slot_weights ? (uint32_t)((n_slot + pk::kGidThreads - 1u) / pk::kGidThreads) : 0u;
-    const uint32_t lds = n <= pk::kGidMarked ? (n + 255u) / 256u * 32u : 0u;
-    hipLaunchKernelGGL(pk::group_ids_kernel, dim3(n_expert + n_shared + copies), dim3(pk::kGidThreads), lds,
-                       pk::stream(), a);
+    const uint32_t n = n_tok * k_used;
+    const uint32_t copies = slot_weights ? (uint32_t)((n_slot + pk::kGidThreads - 1u) / pk::kGidThreads) : 0u;
+    const dim3 grid(n_expert + n_shared + copies), block(pk::kGidThreads);
+    if (n <= 65536u) {
+        hipLaunchKernelGGL(pk::group_ids_kernel<1>, grid, block, 0, pk::stream(), a);
+    } else {
+        a.kept = n <= 8u * 65536u ? 1u : 0u;
+        hipLaunchKernelGGL(pk::group_ids_kernel<8>, grid, block, 0, pk::stream(), a);
+    }
     return pk::launch_ok("moe group ids launch");
 }

@@ -68,10 +68,11 @@ __global__ __launch_bounds__(PK_MV_TPB) void matvec_kernel(float *__restrict__ o
 #pragma unroll
             for (uint32_t t = 0; t < T; t++) {
                 const uint32_t tok = t0 + t < n_tok ? t0 + t : n_tok - 1u;
-                const auto got = epi.get(tok, row_ok ? row : 0u);
+                const float bias = epi.bias_of(row_ok ? row : 0u), res = epi.residual_of(tok, row_ok ? row : 0u);
                 float acc = row_partial<Q, UPLMAX>(row_ok, rg, wu[p], a[t], lut);
                 acc = row_finish(acc, rg);
-                if (row_ok && rg.holds_row() && t0 + t < n_tok) epi.put(out, out_dim, t0 + t, row, acc, got);
+                if (row_ok && rg.holds_row() && t0 + t < n_tok)
+                    epi.put(out, out_dim, t0 + t, row, acc, bias, res);
             }
         }
         base += n_waves * RPW;
@@ -120,7 +121,8 @@ __global__ __launch_bounds__(256) void matvec_wide_kernel(float *__restrict__ ou
 #pragma unroll
     for (uint32_t t = 0; t < T; t++) {
         const float v = row_finish(acc[t], rg);
-        if (rg.holds_row() && t0 + t < n_tok) epi.put(out, out_dim, t0 + t, row, v, epi.get(t0 + t, row));
+        if (rg.holds_row() && t0 + t < n_tok)
+            epi.put(out, out_dim, t0 + t, row, v, epi.bias_of(row), epi.residual_of(t0 + t, row));
     }
 }
 

@@ -133,7 +133,9 @@ PK_DEV void route_token_f64(const GroupRoute &r, uint32_t token, double *c_l) {
             const uint32_t g = (lane * J + j) / size;
             if (g >= 64u || !(kept >> g & 1u)) key[j] = 0ull;
         }
-        __builtin_amdgcn_wave_barrier();  // c_l is read before the wave's next token writes it
+        // c_l is read before the wave's next token writes it
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
     int32_t id = -1;
     double ws = 0.0, sum = 0.0;
@@ -180,6 +182,311 @@ __global__ __launch_bounds__(256) void route_groups_f64_kernel(GroupRoute r) {
     route_token_f64<J>(r, token, c_l[wave]);
 }
 
+
+// ---- four tokens a wave, in f32 with a proof of the order -----------------
+//
+// 16 lanes a token (a DPP row, so that every exchange is a DPP move), lane kk
+// holds experts kk Jr .. kk Jr + Jr - 1. The choice c is taken in f32 and scaled
+// to a 23-bit integer q over a window below the row's best; q, the lane and the
+// expert's place in it make one unique 32-bit key, so that sorting keys is
+// single max / min operations. The error of q is bounded (err), so keys whose q
+// lie `gap` apart are in the order of the 64-bit scores. A row where two
+// neighbours of the result, or the groups at the border, lie closer is done
+// again by route_token_f64, and so is a row that has infinite scores, runs out
+// of candidates or of the window: about one row in a thousand of a trained
+// router's, rows of ties always.
+
+constexpr uint32_t kQShift = 9;  // below q: 15 - kk in 4 bits, 31 - j in 5
+constexpr float kSteps = 8384000.0f;  // q < 2^23, with room for 4600 steps of rounding
+
+// v as an integer, 0 where it is negative or NaN (as the instruction has it)
+PK_DEV uint32_t steps_of(float v) {
+    uint32_t q;
+    asm("v_cvt_u32_f32 %0, %1" : "=v"(q) : "v"(v));
+    return q;
+}
+
+template <uint32_t N>
+struct SortPairs {  // Batcher's odd-even merge sort of N (a power of two)
+    uint32_t n = 0;
+    uint8_t a[N * 8] = {}, b[N * 8] = {};
+    constexpr SortPairs() {
+        for (uint32_t p = 1; p < N; p *= 2)
+            for (uint32_t k = p; k >= 1; k /= 2)
+                for (uint32_t j = k % p; j + k < N; j += 2 * k)
+                    for (uint32_t i = 0; i < k && i + j + k < N; i++)
+                        if ((i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                            a[n] = (uint8_t)(i + j);
+                            b[n++] = (uint8_t)(i + j + k);
+                        }
+    }
+};
+
+PK_DEV uint32_t max_u(uint32_t a, uint32_t b) { return a > b ? a : b; }
+PK_DEV uint32_t min_u(uint32_t a, uint32_t b) { return a < b ? a : b; }
+PK_DEV void falling(uint32_t &a, uint32_t &b) {
+    const uint32_t x = max_u(a, b);
+    b = min_u(a, b);
+    a = x;
+}
+
+template <uint32_t N>
+PK_DEV void sort_falling(uint32_t (&v)[N]) {
+    constexpr SortPairs<N> net;
+#pragma unroll
+    for (uint32_t i = 0; i < net.n; i++) falling(v[net.a[i]], v[net.b[i]]);
+}
+
+// a: the N largest of two falling lists, falling (theirs in place, other(i)
+// element i of the second): the larger ends of the two, one against the other's
+// reverse, are those N, rising then falling; log N steps of exchanges sort them
+template <uint32_t N, typename Other>
+PK_DEV void merge_falling(uint32_t (&a)[N], Other other) {
+    uint32_t o[N];
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) o[i] = other(i);
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) a[i] = max_u(a[i], o[N - 1u - i]);
+#pragma unroll
+    for (uint32_t d = N / 2u; d >= 1u; d /= 2u)
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+            if (!(i & d)) falling(a[i], a[i + d]);
+}
+
+// Reductions over the 16 lanes of a row, the result in all of them
+template <typename T, typename F>
+PK_DEV T row_reduce(T v, F f) {
+#pragma unroll
+    for (uint32_t m = 1; m < 16; m <<= 1)
+        v = f(v, __builtin_bit_cast(T, partner(__builtin_bit_cast(int32_t, v), m)));
+    return v;
+}
+PK_DEV float row_max_f(float v) {
+    return row_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+PK_DEV double row_sum(double v) {
+#pragma unroll
+    for (uint32_t m = 1; m < 16; m <<= 1) {
+        uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)partner((int32_t)(uint32_t)u, m), hi = (uint32_t)partner((int32_t)(u >> 32), m);
+        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    }
+    return v;
+}
+// lane i gets lane (i - N) % 16 of its row
+template <uint32_t N>
+PK_DEV uint32_t row_turn(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xF, 0xF, false);
+}
+// how many of the row's other groups, of G lanes each, have a larger v
+template <uint32_t G, uint32_t N = G>
+PK_DEV uint32_t groups_ahead(uint32_t v) {
+    if constexpr (N >= 16u)
+        return 0u;
+    else
+        return (row_turn<N>(v) > v ? 1u : 0u) + groups_ahead<G, N + G>(v);
+}
+
+// J: experts a lane, 16 J >= n_expert; K: k_used <= K. Groups are whole lanes:
+// n_group divides 16, and 16 n_expert where there are several.
+template <uint32_t J, uint32_t K>
+__global__ __launch_bounds__(256) void route_groups_kernel(GroupRoute r, uint32_t per_lane) {
+    constexpr uint32_t kJ64 = J < 4u ? 1u : J / 4u;
+    // A lane's experts in LDS: rows are read from memory as they lie, 16 lanes
+    // that read J floats each then find them on distinct banks
+    constexpr uint32_t kPitch = J + 4u, kRow = 16u * kPitch;
+    static_assert(4u * kRow * 4u >= 64u * kJ64 * 8u, "route_token_f64's doubles take the rows' place");
+    __shared__ __align__(16) float rows_l[4][4u * kRow];
+    __shared__ __align__(16) float bias_l[kRow];
+    const uint32_t lane = threadIdx.x & 63u, kk = lane & 15u, E = r.n_expert;
+    const uint32_t token0 = (blockIdx.x * 4u + (threadIdx.x >> 6)) * 4u;
+    const uint32_t part = 65536u / per_lane + 1u;  // e / per_lane = e part >> 16 for e < 1024
+    auto place = [&](uint32_t e) {
+        const uint32_t o = e * part >> 16;
+        return o * kPitch + (e - o * per_lane);
+    };
+    float *mine_l = rows_l[threadIdx.x >> 6];
+    if (J >= 4u && E == 16u * J) {  // rows of whole 16-byte pieces, one after the other
+#pragma unroll
+        for (uint32_t i = 0; i < J / 4u; i++) {
+            const uint32_t f = (lane + 64u * i) * 4u, t = f / (16u * J), e = f % (16u * J);
+            const uint32_t token = token0 + t < r.n_tok ? token0 + t : r.n_tok - 1u;
+            *(uint4 *)(mine_l + t * kRow + e / J * kPitch + e % J) =
+                    ld128((const uint8_t *)(r.logits + (uint64_t)token * E + e));
+        }
+    } else {
+        for (uint32_t i = lane; i < 4u * kRow; i += 64u) mine_l[i] = __builtin_nanf("");  // no expert there
+        __builtin_amdgcn_wave_barrier();  // a wave's LDS writes land in order
+        for (uint32_t t = 0; t < 4u; t++) {
+            const uint32_t token = token0 + t < r.n_tok ? token0 + t : r.n_tok - 1u;
+            for (uint32_t e = lane; e < E; e += 64u) mine_l[t * kRow + place(e)] = r.logits[(uint64_t)token * E + e];
+        }
+    }
+    if (r.bias)
+        for (uint32_t e = threadIdx.x; e < E; e += 256u) bias_l[place(e)] = r.bias[e];
+    __syncthreads();
+    if (token0 >= r.n_tok) return;  // whole wave, behind the block's only barrier
+    const uint32_t token = token0 + (lane >> 4);
+    const float *row_l = mine_l + (lane >> 4) * kRow;
+    // c; NaN or -inf for an expert that is no candidate. err: how far c may be
+    // from the exact one, in steps of 2^-24
+    float c[J], err, window;
+    float m = 0.0f, z = 1.0f;
+    bool unsure = false;
+    constexpr float kLog2e = 1.4426950408889634f;
+    const bool by_logit = r.softmax && !r.bias && (r.n_group == 1u || r.group_top == 1u);
+#pragma unroll
+    for (uint32_t j = 0; j < J; j++) {
+        const float l = row_l[kk * kPitch + j];
+        c[j] = l > -INFINITY ? l : __builtin_nanf("");
+    }
+    if (r.softmax) {
+        m = -INFINITY;
+#pragma unroll
+        for (uint32_t j = 0; j < J; j++) m = fmaxf(m, c[j]);
+        m = row_max_f(m);
+        unsure = !(fabsf(m) < INFINITY);
+        float x[J];
+        if (!by_logit || !r.renorm) {
+            float sum[J];
+#pragma unroll
+            for (uint32_t j = 0; j < J; j++) {
+                x[j] = __builtin_amdgcn_exp2f((c[j] - m) * kLog2e);
+                sum[j] = fmaxf(x[j], 0.0f);  // NaN: none
+            }
+#pragma unroll
+            for (uint32_t d = J / 2u; d >= 1u; d /= 2u)
+#pragma unroll
+                for (uint32_t j = 0; j < d; j++) sum[j] += sum[j + d];
+            z = row_reduce(sum[0], [](float a, float b) { return a + b; });
+        }
+        if (by_logit) {  // the softmax keeps their order
+            err = 0.0f;
+            window = 16.0f;
+        } else {
+            // a term e^-x is off by (3 x + 2) steps of itself, at most 2.2 of the
+            // largest, z by the terms' mean of that, at most 3 ln 512 + 2 = 20.7,
+            // and by the 9 additions of a sum; the quotient and the product 2
+            const float rz = 1.0f / z;
+#pragma unroll
+            for (uint32_t j = 0; j < J; j++) c[j] = x[j] * rz;
+            err = 34.0f * rz;
+            window = r.bias ? 1.0f : rz;
+        }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < J; j++)
+            // e^-l off by (2 |l| + 2) steps of itself, which moves s by at most 2;
+            // the sum, the reciprocal and its rounding 4
+            c[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(c[j] * -kLog2e));
+        err = 8.0f;
+        window = r.bias ? 2.0f : 1.0f;
+    }
+    if (r.bias) {
+#pragma unroll
+        for (uint32_t j = 0; j < J; j++) c[j] += bias_l[kk * kPitch + j];
+    }
+    float hi = -INFINITY;
+#pragma unroll
+    for (uint32_t j = 0; j < J; j++) hi = fmaxf(hi, c[j]);
+    hi = row_max_f(hi);
+    unsure |= !(fabsf(hi) < INFINITY);
+    // q = 0: no candidate, or one below the window (a row that needs it is unsure)
+    const float scale = kSteps / window, shift = 2.0f - (hi - window) * scale;
+    if (!by_logit) err += fabsf(hi) + window;
+    unsure |= !(fabsf(shift) < 6e10f);  // its rounding is the whole row's, below 3600 steps
+    // on both sides the error of c, two roundings of a step of q each and its floor
+    const float gap_f = 2.0f * err * 0x1p-24f * scale + 8.0f;
+    const uint32_t gap = gap_f < kSteps ? (uint32_t)gap_f : 1u << 23;
+    constexpr uint32_t N = J < K ? J : K, L = J / N;  // L falling lists of N
+    uint32_t s[L][N];
+#pragma unroll
+    for (uint32_t j = 0; j < J; j++)
+        s[j / N][j % N] = steps_of(__builtin_fmaf(c[j], scale, shift)) << kQShift | (31u - j);
+    uint32_t top[K];
+#pragma unroll
+    for (uint32_t i = 0; i < L; i++) {
+        sort_falling(s[i]);
+        if (i > 0u) merge_falling(s[0], [&](uint32_t k) { return s[i][k]; });
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < K; k++) top[k] = k < N ? s[0][k < N ? k : 0u] | (15u - kk) << 5 : 0u;
+    if (r.n_group > 1u) {
+        const uint32_t lanes = 16u / r.n_group;  // of a group
+        uint32_t g0 = top[0], g1 = K > 1u ? top[K > 1u ? 1 : 0] : 0u;
+#pragma unroll
+        for (uint32_t st = 1; st < 16u; st <<= 1)
+            if (st < lanes) {  // uniform
+                const uint32_t o0 = (uint32_t)partner((int32_t)g0, st), o1 = (uint32_t)partner((int32_t)g1, st);
+                g1 = max_u(max_u(g1, o1), min_u(g0, o0));
+                g0 = max_u(g0, o0);
+            }
+        const bool two = r.group_top == 2u && E > r.n_group;  // a group of one expert is that one
+        const uint32_t q0 = g0 >> kQShift, q1 = g1 >> kQShift, stand = q0 + (two ? q1 : 0u);
+        // a group that stands with one, or with what the window cut, has no sum here
+        unsure |= two && q1 == 0u;
+        const uint32_t ahead = lanes == 2u   ? groups_ahead<2>(stand)
+                               : lanes == 4u ? groups_ahead<4>(stand)
+                               : lanes == 8u ? groups_ahead<8>(stand)
+                                             : groups_ahead<1>(stand);
+        const bool kept = ahead < r.topk_group;
+        const uint64_t all = __ballot(kept);
+        unsure |= (uint32_t)__builtin_popcount((uint32_t)(all >> (lane & 48u)) & 0xffffu) != r.topk_group * lanes;
+        const uint32_t last = row_reduce(kept ? stand : UINT32_MAX, min_u), next = row_reduce(kept ? 0u : stand, max_u);
+        unsure |= r.topk_group < r.n_group && last - next < 2u * gap;
+#pragma unroll
+        for (uint32_t k = 0; k < K; k++) top[k] = kept ? top[k] : 0u;
+    }
+    // the lane's best are kept to see what is left behind the row's
+    uint32_t own[N];
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) own[k] = top[k];
+#pragma unroll
+    for (uint32_t st = 1; st < 16u; st <<= 1)
+        merge_falling(top, [&](uint32_t k) { return (uint32_t)partner((int32_t)top[k], st); });
+    // the last winner, the best one behind it (of a lane's own list, or the place
+    // behind the list's end, which is no larger than its last)
+    uint32_t won = 0u, last = 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < K; k++) {
+        won = kk == k ? top[k] : won;
+        last = k + 1u == r.k_used ? top[k] : last;  // scalar compare
+        if (k > 0u) unsure |= k < r.k_used && (top[k - 1u] >> kQShift) - (top[k] >> kQShift) < gap;
+    }
+    uint32_t next = 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) next = max_u(next, own[k] < last ? own[k] : 0u);
+    next = row_reduce(next, max_u);
+    unsure |= last >> kQShift == 0u || (last >> kQShift) - (next >> kQShift) < gap;
+    // a lane all of whose list won may hold a better one behind it
+    if constexpr (L > 1u) unsure |= own[N - 1u] >= last;
+    const bool here = kk < r.k_used;
+    const uint32_t id = here ? (15u - (won >> 5 & 15u)) * per_lane + 31u - (won & 31u) : 0u;
+    const double raw = (double)row_l[place(id)];
+    double w;
+    if (r.softmax) {
+        w = here ? exp(raw - (double)m) : 0.0;
+        const double total = r.renorm ? row_sum(w) : (double)z;
+        w = total > 0.0 ? w / total : 0.0;  // as far below the row's best as 64 bits reach: 0
+    } else {
+        const double e = exp(-fabs(raw));
+        w = here ? (raw >= 0.0 ? 1.0 : e) / (1.0 + e) : 0.0;
+        if (r.renorm) w /= fmax(row_sum(w), 6.103515625e-5);
+    }
+    const uint64_t slow = __ballot(unsure);
+    if (token < r.n_tok && here && ((slow >> (lane & 48u)) & 0xffffu) == 0u) {
+        r.selected[(uint64_t)token * r.k_used + kk] = (int32_t)id;
+        r.weights[(uint64_t)token * r.k_used + kk] = (float)(w * (double)r.scale);
+    }
+    if (slow == 0ull) return;
+    // the rows are read before doubles take their place
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (uint32_t i = 0; i < 4u && token0 + i < r.n_tok; i++)  // wave-uniform
+        if ((slow >> (16u * i)) & 0xffffu) route_token_f64<kJ64>(r, token0 + i, (double *)mine_l);
+}
+
 }  // namespace pk
 
 extern "C" int pulsar_router_select_groups(void *selected, void *weights, const void *logits, const void *bias,
@@ -193,6 +500,35 @@ extern "C" int pulsar_router_select_groups(void *selected, void *weights, const 
         return pk::reject("router select groups");
     const pk::GroupRoute r = {(const float *)logits, (const float *)bias, (int32_t *)selected, (float *)weights,
                               n_expert, k_used, n_group, topk_group, group_top, score, renorm, n_tok, weight_scale};
+    // whole lanes of the 16 a token has: the f32 kernel
+    if (n_expert <= 512u && k_used <= 16u && 16u % n_group == 0u && (n_group == 1u || n_expert % 16u == 0u)) {
+        const uint32_t per_lane = (n_expert + 15u) / 16u;
+        const dim3 blocks((n_tok + 15u) / 16u);
+#define PK_RGFK(J, K)                                                                                          \
+    hipLaunchKernelGGL((pk::route_groups_kernel<J, K>), blocks, dim3(256), 0, pk::stream(), r, per_lane)
+#define PK_RGF(J)             \
+    do {                      \
+        if (k_used <= 8u)     \
+            PK_RGFK(J, 8);    \
+        else                  \
+            PK_RGFK(J, 16);   \
+    } while (0)
+        if (per_lane <= 1u)
+            PK_RGF(1);
+        else if (per_lane <= 2u)
+            PK_RGF(2);
+        else if (per_lane <= 4u)
+            PK_RGF(4);
+        else if (per_lane <= 8u)
+            PK_RGF(8);
+        else if (per_lane <= 16u)
+            PK_RGF(16);
+        else
+            PK_RGF(32);
+#undef PK_RGF
+#undef PK_RGFK
+        return pk::launch_ok("router select groups launch");
+    }
     const dim3 grid((n_tok + 3u) / 4u);
 #define PK_RG64(J) hipLaunchKernelGGL(pk::route_groups_f64_kernel<J>, grid, dim3(256), 0, pk::stream(), r)
     if (n_expert <= 64u)

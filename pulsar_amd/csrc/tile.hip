@@ -30,23 +30,34 @@ __global__ __launch_bounds__(256, 2) void tile_gemm_kernel(float *__restrict__ o
     if (item >= n_item) return;  // block-uniform
     const uint32_t t0 = (item % n_tt) * T::kTok;
     const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, wave = threadIdx.x >> 6;
-    const uint32_t row = (item / n_tt * WR + wave % WR) * 32u + (lane & 15u);
+    uint32_t row = (item / n_tt * WR + wave % WR) * 32u + (lane & 15u);
     const uint32_t np = n_tok - t0 < T::kTok ? n_tok - t0 : T::kTok;
     auto wrow = [&](uint32_t r) { return w + (uint64_t)(r < out_dim ? r : out_dim - 1u) * row_bytes; };
     T tile;
     tile.run(buf0, buf1, lut, wrow(row), wrow(row + 16u), nb, np, (const uint8_t *)(xq + (uint64_t)t0 * nb),
              [&](uint32_t t) { return t * (nb * 292u); });
+    // nothing of the epilogue is fetched or formed before here: the tile has no registers for it
+    asm volatile("" : "+v"(row) : : "memory");
+    const uint32_t at[2] = {row < out_dim ? row : out_dim - 1u, row + 16u < out_dim ? row + 16u : out_dim - 1u};
+    const float bias[2] = {epi.bias_of(at[0]), epi.bias_of(at[1])};
 #pragma unroll
-    for (uint32_t n = 0; n < NS; n++)
+    for (uint32_t n = 0; n < NS; n++) {
+        float res[4][2];
+#pragma unroll
+        for (uint32_t r = 0; r < 4; r++)
+            if (T::mine(n, r, wave / WR)) {
+                const uint32_t t = 16u * n + 4u * q + r, tc = t0 + (t < np ? t : np - 1u);
+                res[r][0] = epi.residual_of(tc, at[0]);
+                res[r][1] = epi.residual_of(tc, at[1]);
+            }
 #pragma unroll
         for (uint32_t r = 0; r < 4; r++) {
             const uint32_t t = 16u * n + 4u * q + r;
             if (!T::mine(n, r, wave / WR) || t >= np) continue;
-            const auto got0 = epi.get(t0 + t, row < out_dim ? row : out_dim - 1u);
-            const auto got1 = epi.get(t0 + t, row + 16u < out_dim ? row + 16u : out_dim - 1u);
-            if (row < out_dim) epi.put(out, out_dim, t0 + t, row, tile.acc[n][0][r], got0);
-            if (row + 16u < out_dim) epi.put(out, out_dim, t0 + t, row + 16u, tile.acc[n][1][r], got1);
+            if (row < out_dim) epi.put(out, out_dim, t0 + t, row, tile.acc[n][0][r], bias[0], res[r][0]);
+            if (row + 16u < out_dim) epi.put(out, out_dim, t0 + t, row + 16u, tile.acc[n][1][r], bias[1], res[r][1]);
         }
+    }
 }
 
 template <uint32_t Q, uint32_t WR, uint32_t WK, uint32_t NS>

@@ -55,31 +55,38 @@ def matmul_kq(out, w, xq, in_dim: int, out_dim: int, n_tok: int, row_bytes: int,
     )
 
 
-def _room(buf, nbytes: int, op: str, what: str) -> int:
+def _room(buf, nbytes: int, op: str, what: str, device: int) -> int:
     """The device address of `buf`, which the launch uses the first nbytes
     bytes of; a tensor has to be contiguous, that large and on the current
     device (a raw address is the caller's word for all three)."""
-    if buf is None or isinstance(buf, int) or not hasattr(buf, "data_ptr"):
+    if buf is None or not hasattr(buf, "data_ptr"):
         return _ptr(buf)
-    at = _ptr(buf)
-    if not buf.is_contiguous() or buf.numel() * buf.element_size() < nbytes:
+    if buf.get_device() != device:
+        _misplaced(buf, op, what)
+    if buf.nbytes < nbytes or not buf.is_contiguous():
         raise ValueError(f"{op}: {what} has to be contiguous and hold {nbytes} bytes")
-    _same_device(buf, op, what)
-    return at
+    return buf.data_ptr()
 
 
-def _same_device(buf, op: str, what: str) -> None:
-    if buf.get_device() != _lib.torch.cuda.current_device():
-        raise ValueError(f"{op}: {what} is not on the current device")
+def _misplaced(buf, op: str, what: str) -> None:
+    _ptr(buf)  # a host tensor
+    raise ValueError(f"{op}: {what} is not on the current device")
 
 
-def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str) -> int:
+def _device() -> int:
+    """The current device, -2 (no tensor's) before the GPU is first used."""
+    cuda = _lib.torch.cuda
+    return cuda.current_device() if cuda.is_initialized() else -2
+
+
+def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str, device: int) -> int:
     """The device address of n_rows rows of dim floats, `stride` floats apart.
     A tensor may be a view of columns of a wider array: it has to be f32 [..,
     dim] with that stride, or contiguous and large enough."""
-    if buf is None or isinstance(buf, int) or not hasattr(buf, "data_ptr"):
+    if buf is None or not hasattr(buf, "data_ptr"):
         return _ptr(buf)
-    at = _ptr(buf)
+    if buf.get_device() != device:
+        _misplaced(buf, op, what)
     if buf.element_size() != 4:
         raise ValueError(f"{op}: {what} has to be f32")
     if buf.is_contiguous():
@@ -89,8 +96,7 @@ def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str) -> int:
               and buf.stride(0) == stride)
     if not ok:
         raise ValueError(f"{op}: {what} has to hold {n_rows} rows of {dim} f32 values {stride} apart")
-    _same_device(buf, op, what)
-    return at
+    return buf.data_ptr()
 
 
 def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok: int, row_bytes: int, quant: int,
@@ -98,13 +104,13 @@ def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok
     """matmul_kq with its epilogue in the same launch: out[t] = act(W x_t +
     bias) + residual[t] (formats.EPI_* codes; bias and residual may be None).
     Strides in floats, 0 for packed rows; residual may be out itself."""
-    op = "matmul_kq_fused"
+    op, dev = "matmul_kq_fused", _device()
     xq_bytes, so, sr = n_tok * -(-in_dim // 256) * 292, out_stride or out_dim, res_stride or out_dim
     _check(
         _lib.load().pulsar_matmul_kq_fused(
-            _rows(out, n_tok, out_dim, so, op, "out"), _room(w, (out_dim - 1) * row_bytes, op, "w"),
-            _room(xq, xq_bytes, op, "xq"), _room(bias, 4 * out_dim, op, "bias"),
-            _rows(residual, n_tok, out_dim, sr, op, "residual"), in_dim, out_dim, n_tok, row_bytes, quant, act,
+            _rows(out, n_tok, out_dim, so, op, "out", dev), _room(w, (out_dim - 1) * row_bytes, op, "w", dev),
+            _room(xq, xq_bytes, op, "xq", dev), _room(bias, 4 * out_dim, op, "bias", dev),
+            _rows(residual, n_tok, out_dim, sr, op, "residual", dev), in_dim, out_dim, n_tok, row_bytes, quant, act,
             out_stride, res_stride),
         op,
     )
@@ -184,12 +190,13 @@ def router_select_groups(selected, weights, logits, bias, n_expert: int, k_used:
     """Top-k of the experts of the topk_group best of n_group expert groups
     (a group's score: its group_top largest score + bias; formats.SCORE_*),
     the weights the winners' scores, renormalised if renorm, times weight_scale."""
-    op = "router_select_groups"
+    op, dev = "router_select_groups", _device()
     _check(
         _lib.load().pulsar_router_select_groups(
-            _room(selected, 4 * n_tok * k_used, op, "selected"), _room(weights, 4 * n_tok * k_used, op, "weights"),
-            _room(logits, 4 * n_tok * n_expert, op, "logits"), _room(bias, 4 * n_expert, op, "bias"), n_expert, k_used,
-            n_group, topk_group, group_top, score, int(bool(renorm)), weight_scale, n_tok),
+            _room(selected, 4 * n_tok * k_used, op, "selected", dev),
+            _room(weights, 4 * n_tok * k_used, op, "weights", dev),
+            _room(logits, 4 * n_tok * n_expert, op, "logits", dev), _room(bias, 4 * n_expert, op, "bias", dev), n_expert,
+            k_used, n_group, topk_group, group_top, score, int(bool(renorm)), weight_scale, n_tok),
         op,
     )
 
@@ -247,15 +254,16 @@ def moe_group_ids(gptrs, starts, pairs, slot_weights, selected, router_weights, 
     is bank expert e, then one group per shared slot; the grouped stages take it
     with n_group = n_expert + len(shared). slot_weights (None: left out) gets
     router_weights and the shared slots' ones."""
-    op = "moe_group_ids"
+    op, dev = "moe_group_ids", _device()
     arr, n_shared = _shared_array(shared)
     groups, slots = n_expert + n_shared, k_used + n_shared
     _check(
         _lib.load().pulsar_moe_group_ids(
-            _room(gptrs, EXPERT_PTRS_BYTES * groups, op, "gptrs"), _room(starts, 4 * (groups + 1), op, "starts"),
-            _room(pairs, 4 * n_tok * slots, op, "pairs"), _room(slot_weights, 4 * n_tok * slots, op, "slot_weights"),
-            _room(selected, 4 * n_tok * k_used, op, "selected"),
-            _room(router_weights, 4 * n_tok * k_used, op, "router_weights"), ctypes.byref(bank), n_expert,
+            _room(gptrs, EXPERT_PTRS_BYTES * groups, op, "gptrs", dev),
+            _room(starts, 4 * (groups + 1), op, "starts", dev), _room(pairs, 4 * n_tok * slots, op, "pairs", dev),
+            _room(slot_weights, 4 * n_tok * slots, op, "slot_weights", dev),
+            _room(selected, 4 * n_tok * k_used, op, "selected", dev),
+            _room(router_weights, 4 * n_tok * k_used, op, "router_weights", dev), ctypes.byref(bank), n_expert,
             ctypes.cast(arr, ctypes.c_void_p), n_shared, n_tok, k_used),
         op,
     )

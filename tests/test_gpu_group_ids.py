@@ -95,10 +95,11 @@ def test_one_expert_takes_all(dev):
     check(dev, np.full((5000, 4), 3, np.int32), 8, 0)
 
 
-def test_more_ids_than_the_marks_hold(dev):
-    """Above 262,144 ids the blocks read them twice; the ids of this chunk are
-    checked by numpy's stable sort."""
-    T, k, experts = 40001, 7, 96
+@pytest.mark.parametrize("T,k", [(30001, 3), (80001, 6), (80001, 7), (65536, 8), (65537, 8), (131072, 8)])
+def test_long_chunks(dev, T, k):
+    """Chunks whose marks take several registers and, above 524,288 ids, that the
+    blocks read twice; checked by numpy's stable sort."""
+    experts = 96
     ids = np.random.default_rng(2).integers(-1, experts, (T, k)).astype(np.int32)
     gptrs = torch.zeros((experts, 6), dtype=torch.int64, device=dev)
     starts = torch.zeros(experts + 1, dtype=torch.int32, device=dev)
