@@ -14,6 +14,10 @@
 
 namespace pk {
 
+#ifndef PK_RG_MANY
+#define PK_RG_MANY 4096u
+#endif
+
 constexpr uint32_t kMaxGroups = 64;
 
 struct GroupRoute {
@@ -49,13 +53,10 @@ PK_DEV double wave_sum(double v) {
     for (uint32_t m = 1; m < 64; m <<= 1) v += __shfl_xor(v, (int)m, 64);
     return v;
 }
-PK_DEV uint64_t wave_max_u64(uint64_t v) {
-#pragma unroll
-    for (uint32_t m = 1; m < 64; m <<= 1) {
-        const uint64_t o = __shfl_xor((unsigned long long)v, (int)m, 64);
-        v = v > o ? v : o;
-    }
-    return v;
+PK_DEV uint64_t wave_max_u64(uint64_t v) {  // the largest high word, then of those the largest low one
+    const uint32_t hi = wave_max_u32((uint32_t)(v >> 32));
+    const uint32_t lo = wave_max_u32((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return (uint64_t)hi << 32 | lo;
 }
 
 // One token by one wave, everything in 64 bits: lane l holds experts lJ .. lJ
@@ -111,27 +112,35 @@ PK_DEV void route_token_f64(const GroupRoute &r, uint32_t token, double *c_l) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        // lane g: group g's two largest, then its rank among the groups
+        // `of` lanes a group (a power of two), each the two largest of its share
+        uint32_t of = 64u / r.n_group;
+        of = 1u << (31 - __builtin_clz(of));
+        const uint32_t g = lane / of, first = lane % of;
         double c0 = -INFINITY, c1 = -INFINITY;
-        if (lane < r.n_group)
-            for (uint32_t i = 0; i < size; i++) {
-                const double v = c_l[lane * size + i];
+        if (g < r.n_group)
+            for (uint32_t i = first; i < size; i += of) {
+                const double v = c_l[g * size + i];
                 c1 = fmax(c1, fmin(c0, v));
                 c0 = fmax(c0, v);
             }
+        for (uint32_t m = 1; m < of; m <<= 1) {
+            const double o0 = __shfl_xor(c0, (int)m, 64), o1 = __shfl_xor(c1, (int)m, 64);
+            c1 = fmax(fmax(c1, o1), fmin(c0, o0));
+            c0 = fmax(c0, o0);
+        }
         // a group of one candidate stands with that one, a group of none behind all
         const double gs = r.group_top == 2u && c1 > -INFINITY ? c0 + c1 : c0;
         const uint64_t gk = c0 > -INFINITY ? order_key(gs) : 0ull;
         uint32_t rank = 0;
         for (uint32_t h = 0; h < r.n_group; h++) {
-            const uint64_t o = lane_bcast(gk, h);
-            rank += o > gk || (o == gk && h < lane) ? 1u : 0u;
+            const uint64_t o = lane_bcast(gk, h * of);
+            rank += o > gk || (o == gk && h < g) ? 1u : 0u;
         }
-        const uint64_t kept = __ballot(lane < r.n_group && rank < r.topk_group);
+        const uint64_t kept = __ballot(g < r.n_group && rank < r.topk_group);  // bit g of: group g
 #pragma unroll
         for (uint32_t j = 0; j < J; j++) {
-            const uint32_t g = (lane * J + j) / size;
-            if (g >= 64u || !(kept >> g & 1u)) key[j] = 0ull;
+            const uint32_t at = (lane * J + j) / size * of;
+            if (at >= 64u || !(kept >> at & 1u)) key[j] = 0ull;
         }
         // c_l is read before the wave's next token writes it
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -190,11 +199,13 @@ __global__ __launch_bounds__(256) void route_groups_f64_kernel(GroupRoute r) {
 // to a 23-bit integer q over a window below the row's best; q, the lane and the
 // expert's place in it make one unique 32-bit key, so that sorting keys is
 // single max / min operations. The error of q is bounded (err), so keys whose q
-// lie `gap` apart are in the order of the 64-bit scores. A row where two
-// neighbours of the result, or the groups at the border, lie closer is done
-// again by route_token_f64, and so is a row that has infinite scores, runs out
-// of candidates or of the window: about one row in a thousand of a trained
-// router's, rows of ties always.
+// lie `gap` apart are in the order of the 64-bit scores. That settles which
+// experts win; the winners, and the one behind them if it is close, are then put
+// to the test by their 64-bit scores. A row that fails it (ties, an order that
+// f32 swapped), whose groups at the border lie closer than the gap, that has
+// infinite scores or runs out of candidates or of the window, is done again by
+// route_token_f64: of a trained router's rows one in some thousands, rows of ties
+// always.
 
 constexpr uint32_t kQShift = 9;  // below q: 15 - kk in 4 bits, 31 - j in 5
 constexpr float kSteps = 8384000.0f;  // q < 2^23, with room for 4600 steps of rounding
@@ -274,6 +285,13 @@ PK_DEV double row_sum(double v) {
     }
     return v;
 }
+// lane i gets lane i + 1 of its row
+PK_DEV double row_behind(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x101, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), 0x101, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 // lane i gets lane (i - N) % 16 of its row
 template <uint32_t N>
 PK_DEV uint32_t row_turn(uint32_t v) {
@@ -290,17 +308,19 @@ PK_DEV uint32_t groups_ahead(uint32_t v) {
 
 // J: experts a lane, 16 J >= n_expert; K: k_used <= K. Groups are whole lanes:
 // n_group divides 16, and 16 n_expert where there are several.
-template <uint32_t J, uint32_t K>
-__global__ __launch_bounds__(256) void route_groups_kernel(GroupRoute r, uint32_t per_lane) {
+// W: waves of a block (blocks start at about one in 4 ns, so a long chunk takes
+// few large ones).
+template <uint32_t J, uint32_t K, uint32_t W>
+__global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint32_t per_lane) {
     constexpr uint32_t kJ64 = J < 4u ? 1u : J / 4u;
     // A lane's experts in LDS: rows are read from memory as they lie, 16 lanes
     // that read J floats each then find them on distinct banks
     constexpr uint32_t kPitch = J + 4u, kRow = 16u * kPitch;
     static_assert(4u * kRow * 4u >= 64u * kJ64 * 8u, "route_token_f64's doubles take the rows' place");
-    __shared__ __align__(16) float rows_l[4][4u * kRow];
+    __shared__ __align__(16) float rows_l[W][4u * kRow];
     __shared__ __align__(16) float bias_l[kRow];
     const uint32_t lane = threadIdx.x & 63u, kk = lane & 15u, E = r.n_expert;
-    const uint32_t token0 = (blockIdx.x * 4u + (threadIdx.x >> 6)) * 4u;
+    const uint32_t token0 = (blockIdx.x * W + (threadIdx.x >> 6)) * 4u;
     const uint32_t part = 65536u / per_lane + 1u;  // e / per_lane = e part >> 16 for e < 1024
     auto place = [&](uint32_t e) {
         const uint32_t o = e * part >> 16;
@@ -324,7 +344,7 @@ __global__ __launch_bounds__(256) void route_groups_kernel(GroupRoute r, uint32_
         }
     }
     if (r.bias)
-        for (uint32_t e = threadIdx.x; e < E; e += 256u) bias_l[place(e)] = r.bias[e];
+        for (uint32_t e = threadIdx.x; e < E; e += 64u * W) bias_l[place(e)] = r.bias[e];
     __syncthreads();
     if (token0 >= r.n_tok) return;  // whole wave, behind the block's only barrier
     const uint32_t token = token0 + (lane >> 4);
@@ -445,34 +465,57 @@ __global__ __launch_bounds__(256) void route_groups_kernel(GroupRoute r, uint32_
 #pragma unroll
     for (uint32_t st = 1; st < 16u; st <<= 1)
         merge_falling(top, [&](uint32_t k) { return (uint32_t)partner((int32_t)top[k], st); });
-    // the last winner, the best one behind it (of a lane's own list, or the place
-    // behind the list's end, which is no larger than its last)
+    // winner k to lane k, the last one to all
     uint32_t won = 0u, last = 0u;
 #pragma unroll
     for (uint32_t k = 0; k < K; k++) {
         won = kk == k ? top[k] : won;
         last = k + 1u == r.k_used ? top[k] : last;  // scalar compare
-        if (k > 0u) unsure |= k < r.k_used && (top[k - 1u] >> kQShift) - (top[k] >> kQShift) < gap;
     }
-    uint32_t next = 0u;
+    // the best two keys behind the winners; a lane whose whole list is ahead of
+    // them may hold a better one behind it
+    uint32_t next = 0u, then = 0u;
 #pragma unroll
     for (uint32_t k = 0; k < N; k++) next = max_u(next, own[k] < last ? own[k] : 0u);
     next = row_reduce(next, max_u);
-    unsure |= last >> kQShift == 0u || (last >> kQShift) - (next >> kQShift) < gap;
-    // a lane all of whose list won may hold a better one behind it
-    if constexpr (L > 1u) unsure |= own[N - 1u] >= last;
-    const bool here = kk < r.k_used;
-    const uint32_t id = here ? (15u - (won >> 5 & 15u)) * per_lane + 31u - (won & 31u) : 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) then = max_u(then, own[k] < next ? own[k] : 0u);
+    then = row_reduce(then, max_u);
+    unsure |= last >> kQShift == 0u;
+    if constexpr (L > 1u) unsure |= own[N - 1u] >= next && own[N - 1u] != 0u;
+    const bool close = (last >> kQShift) - (next >> kQShift) < gap;
+    const bool crowd = (last >> kQShift) - (then >> kQShift) < gap;
+    // The winners are known but for `next`, if it is close to the last of them;
+    // lane k_used takes it. Then the order by 64-bit scores, which the weights
+    // take anyway (p + b, whose sum is f32's, by the keys alone)
+    won = kk == r.k_used ? next : won;
+    const bool here = kk < r.k_used, seen = kk <= r.k_used;
+    const uint32_t id = seen ? (15u - (won >> 5 & 15u)) * per_lane + 31u - (won & 31u) : 0u;
     const double raw = (double)row_l[place(id)];
     double w;
     if (r.softmax) {
-        w = here ? exp(raw - (double)m) : 0.0;
-        const double total = r.renorm ? row_sum(w) : (double)z;
-        w = total > 0.0 ? w / total : 0.0;  // as far below the row's best as 64 bits reach: 0
+        w = exp(raw - (double)m);
     } else {
         const double e = exp(-fabs(raw));
-        w = here ? (raw >= 0.0 ? 1.0 : e) / (1.0 + e) : 0.0;
-        if (r.renorm) w /= fmax(row_sum(w), 6.103515625e-5);
+        w = (raw >= 0.0 ? 1.0 : e) / (1.0 + e);
+    }
+    if (by_logit || !r.softmax) {
+        const double choice = w + (r.bias ? (double)bias_l[place(id)] : 0.0);
+        const bool ahead = choice - row_behind(choice) > 1e-15 * fabs(choice);
+        unsure |= kk + 1u < r.k_used && !ahead;
+        unsure |= close && kk + 1u == r.k_used && (kk == 15u || crowd || !ahead);
+    } else {
+        unsure |= close;
+#pragma unroll
+        for (uint32_t k = 1; k < K; k++)
+            unsure |= k < r.k_used && (top[k - 1u] >> kQShift) - (top[k] >> kQShift) < gap;
+    }
+    w = here ? w : 0.0;
+    if (r.softmax) {
+        const double total = r.renorm ? row_sum(w) : (double)z;
+        w = total > 0.0 ? w / total : 0.0;  // as far below the row's best as 64 bits reach: 0
+    } else if (r.renorm) {
+        w /= fmax(row_sum(w), 6.103515625e-5);
     }
     const uint64_t slow = __ballot(unsure);
     if (token < r.n_tok && here && ((slow >> (lane & 48u)) & 0xffffu) == 0u) {
@@ -503,15 +546,21 @@ extern "C" int pulsar_router_select_groups(void *selected, void *weights, const 
     // whole lanes of the 16 a token has: the f32 kernel
     if (n_expert <= 512u && k_used <= 16u && 16u % n_group == 0u && (n_group == 1u || n_expert % 16u == 0u)) {
         const uint32_t per_lane = (n_expert + 15u) / 16u;
-        const dim3 blocks((n_tok + 15u) / 16u);
-#define PK_RGFK(J, K)                                                                                          \
-    hipLaunchKernelGGL((pk::route_groups_kernel<J, K>), blocks, dim3(256), 0, pk::stream(), r, per_lane)
-#define PK_RGF(J)             \
-    do {                      \
-        if (k_used <= 8u)     \
-            PK_RGFK(J, 8);    \
-        else                  \
-            PK_RGFK(J, 16);   \
+        const bool many = n_tok >= PK_RG_MANY;
+#define PK_RGFK(J, K, W)                                                                                       \
+    hipLaunchKernelGGL((pk::route_groups_kernel<J, K, W>), dim3((n_tok + 4u * W - 1u) / (4u * W)), dim3(64u * W), 0, \
+                       pk::stream(), r, per_lane)
+#define PK_RGF(J)                               \
+    do {                                        \
+        constexpr uint32_t kW = J > 16 ? 8 : 16; \
+        if (k_used <= 8u && many)               \
+            PK_RGFK(J, 8, kW);                  \
+        else if (k_used <= 8u)                  \
+            PK_RGFK(J, 8, 4);                   \
+        else if (many)                          \
+            PK_RGFK(J, 16, kW);                 \
+        else                                    \
+            PK_RGFK(J, 16, 4);                  \
     } while (0)
         if (per_lane <= 1u)
             PK_RGF(1);

@@ -95,22 +95,54 @@ def test_one_expert_takes_all(dev):
     check(dev, np.full((5000, 4), 3, np.int32), 8, 0)
 
 
-@pytest.mark.parametrize("T,k", [(30001, 3), (80001, 6), (80001, 7), (65536, 8), (65537, 8), (131072, 8)])
-def test_long_chunks(dev, T, k):
-    """Chunks whose marks take several registers and, above 524,288 ids, that the
-    blocks read twice; checked by numpy's stable sort."""
-    experts = 96
-    ids = np.random.default_rng(2).integers(-1, experts, (T, k)).astype(np.int32)
-    gptrs = torch.zeros((experts, 6), dtype=torch.int64, device=dev)
-    starts = torch.zeros(experts + 1, dtype=torch.int32, device=dev)
-    pairs = torch.full((T * k,), -5, dtype=torch.int32, device=dev)
-    K.moe_group_ids(gptrs, starts, pairs, None, torch.from_numpy(ids).to(dev), None, bank_of(False), experts, [], T, k)
+def want_long(ids, experts, n_shared):
+    """want_groups for long chunks, by numpy's stable sort."""
+    T, k = ids.shape
     flat = ids.reshape(-1)
     order = np.argsort(flat, kind="stable")
-    order = order[flat[order] >= 0]
-    n = len(order)
-    assert np.array_equal(down(starts), np.searchsorted(flat[order], np.arange(experts + 1)))
-    assert np.array_equal(down(pairs)[:n], (order // k) << 4 | order % k) and (down(pairs)[n:] == -5).all()
+    order = order[(flat[order] >= 0) & (flat[order] < experts)]
+    starts = np.searchsorted(flat[order], np.arange(experts + 1))
+    token = np.arange(T)
+    pairs = np.concatenate([(order // k) << 4 | order % k] + [token << 4 | k + i for i in range(n_shared)])
+    return np.concatenate([starts, starts[-1] + T * np.arange(1, n_shared + 1)]), pairs
+
+
+@pytest.mark.parametrize("T,k,experts,n_shared,kind", [
+    (30001, 3, 96, 0, "even"), (80001, 6, 96, 1, "even"), (80001, 7, 96, 0, "even"), (65536, 8, 96, 0, "even"),
+    (65537, 8, 96, 0, "none"), (131072, 8, 96, 0, "even"), (16384, 8, 256, 0, "even"), (16383, 12, 1024, 4, "even"),
+    (9000, 8, 1, 2, "one"), (70000, 1, 1000, 3, "one"), (20000, 8, 8, 1, "skewed"), (5462, 12, 33, 1, "skewed"),
+    (5461, 12, 512, 0, "even"), (4096, 16, 300, 0, "skewed"), (4097, 16, 300, 0, "skewed"), (66000, 1, 2, 0, "last")])
+def test_long_chunks(dev, T, k, experts, n_shared, kind):
+    """Chunks on both sides of the length from which the grouping takes two
+    launches, up to a million ids: even, uneven, one expert's, none's."""
+    rng = np.random.default_rng(T)
+    ids = rng.integers(-1, experts + 1, (T, k)).astype(np.int32)
+    if kind == "one":
+        ids[:] = experts - 1
+    elif kind == "none":
+        ids[:] = -1
+    elif kind == "skewed":
+        ids[rng.random((T, k)) < 0.9] = experts // 3
+    elif kind == "last":
+        ids[:-1] = experts
+    groups = experts + n_shared
+    shared = [tuple((7 << 40) + 16 * (3 * i + j) for j in range(3)) for i in range(n_shared)]
+    want_starts, want_pairs = want_long(ids, experts, n_shared)
+    rw = rng.random((T, k)).astype(np.float32)
+    for _ in range(2):
+        gptrs = torch.full((groups + 1, 6), -5, dtype=torch.int64, device=dev)
+        starts = torch.full((groups + 2,), -5, dtype=torch.int32, device=dev)
+        pairs = torch.full((T * (k + n_shared) + 1,), -5, dtype=torch.int32, device=dev)
+        sw = torch.full((T * (k + n_shared) + 1,), -5.0, device=dev)
+        K.moe_group_ids(gptrs, starts, pairs, sw, torch.from_numpy(ids).to(dev), up_f32(rw), bank_of(False), experts,
+                        shared, T, k)
+        n, p = len(want_pairs), down(pairs)
+        assert np.array_equal(down(starts)[:-1], want_starts) and down(starts)[-1] == -5
+        assert np.array_equal(p[:n], want_pairs) and (p[n:] == -5).all()
+        assert np.array_equal(down(gptrs)[:-1].view(np.uint64), want_ptrs(experts, shared, False))
+        assert (down(gptrs)[-1] == -5).all()
+        want = np.concatenate([rw, np.ones((T, n_shared), np.float32)], 1).reshape(-1)
+        assert np.array_equal(down(sw)[:-1], want) and down(sw)[-1] == -5.0
 
 
 def test_matches_group_csr(dev):
@@ -132,8 +164,9 @@ def test_matches_group_csr(dev):
     assert out[0] == out[1]
 
 
-def test_captured(dev):
-    T, k, E = 700, 4, 40
+@pytest.mark.parametrize("T", [700, 20000])
+def test_captured(dev, T):
+    k, E = 4, 40
     rng = np.random.default_rng(9)
     sel = torch.zeros((T, k), dtype=torch.int32, device=dev)
     g = torch.zeros((E + 1, 6), dtype=torch.int64, device=dev)
@@ -147,7 +180,7 @@ def test_captured(dev):
         torch.cuda.synchronize()
         graph.launch()
         runtime.sync()
-        starts, pairs = want_groups(ids, E, 1)
+        starts, pairs = want_long(ids, E, 1)
         assert np.array_equal(down(s), starts) and np.array_equal(down(p), pairs)
 
 
