@@ -49,6 +49,17 @@ __global__ __launch_bounds__(PK_MV_TPB) void matvec_kernel(float *__restrict__ o
     uint32_t base = (blockIdx.x * waves + threadIdx.x / 64u) * RPW;
     if (base >= n_pass) return;  // whole wave
     typename Fmt<Q>::W wu[RPW][UPLMAX];
+    typename E::Term term[RPW][T];
+    auto fetch = [&] {
+#pragma unroll
+        for (uint32_t p = 0; p < RPW; p++) {
+            const uint32_t row = (base + p) * rpp + rg.rip;
+#pragma unroll
+            for (uint32_t t = 0; t < T; t++)
+                term[p][t] = epi.fetch(t0 + t < n_tok ? t0 + t : n_tok - 1u, row < out_dim ? row : 0u);
+        }
+    };
+    fetch();
 #pragma unroll
     for (uint32_t p = 0; p < RPW; p++) {
         const uint32_t row = (base + p) * rpp + rg.rip;
@@ -67,16 +78,15 @@ __global__ __launch_bounds__(PK_MV_TPB) void matvec_kernel(float *__restrict__ o
             const bool row_ok = row < out_dim;
 #pragma unroll
             for (uint32_t t = 0; t < T; t++) {
-                const uint32_t tok = t0 + t < n_tok ? t0 + t : n_tok - 1u;
-                const float bias = epi.bias_of(row_ok ? row : 0u), res = epi.residual_of(tok, row_ok ? row : 0u);
                 float acc = row_partial<Q, UPLMAX>(row_ok, rg, wu[p], a[t], lut);
                 acc = row_finish(acc, rg);
                 if (row_ok && rg.holds_row() && t0 + t < n_tok)
-                    epi.put(out, out_dim, t0 + t, row, acc, bias, res);
+                    epi.put(out, out_dim, t0 + t, row, acc, term[p][t]);
             }
         }
         base += n_waves * RPW;
         if (base >= n_pass) break;
+        fetch();
 #pragma unroll
         for (uint32_t p = 0; p < RPW; p++) {
             const uint32_t row = (base + p) * rpp + rg.rip;
@@ -122,7 +132,7 @@ __global__ __launch_bounds__(256) void matvec_wide_kernel(float *__restrict__ ou
     for (uint32_t t = 0; t < T; t++) {
         const float v = row_finish(acc[t], rg);
         if (rg.holds_row() && t0 + t < n_tok)
-            epi.put(out, out_dim, t0 + t, row, v, epi.bias_of(row), epi.residual_of(t0 + t, row));
+            epi.put(out, out_dim, t0 + t, row, v, epi.fetch(t0 + t, row));
     }
 }
 
@@ -281,9 +291,6 @@ extern "C" int pulsar_matmul_kq_fused(void *out, const void *w, const void *xq, 
         pk::overlap(out, out_bytes, xq, xq_bytes) || pk::overlap(out, out_bytes, w, (pk::u128)out_dim * row_bytes) ||
         (bias && pk::overlap(out, out_bytes, bias, 4 * (pk::u128)out_dim)))
         return pk::reject("matmul_kq_fused (overlap)");
-    // what is left out is read from xq, which has at least a q8_K block
-    const pk::FusedOut epi = {bias ? (const float *)bias : (const float *)xq,
-                              residual ? (const float *)residual : (const float *)xq, out_stride, res_stride, act,
-                              bias ? 1u : 0u, residual ? 1u : 0u};
+    const pk::FusedOut epi = {(const float *)bias, (const float *)residual, out_stride, res_stride, act};
     return pk::dense_product("matmul_kq_fused (quant)", out, w, xq, in_dim, out_dim, n_tok, row_bytes, quant, epi);
 }

@@ -485,12 +485,12 @@ __global__ __launch_bounds__(64 * RT * C) void mmq_gemm_kernel(float *__restrict
     for (uint32_t e = tid; e < TOK * ROWS; e += NTH) {
         const uint32_t row = e % ROWS, tok = e / ROWS;
         if (r0 + row < out_dim && t0 + tok < n_tok) {
-            const float bias = epi.bias_of(r0 + row), res = epi.residual_of(t0 + tok, r0 + row);
+            const auto term = epi.fetch(t0 + tok, r0 + row);
             const uint32_t prt = row / 16u;
             float v = part[((prt * C) * 16u + row % 16u) * (TOK + 1u) + tok];
 #pragma unroll
             for (uint32_t k = 1; k < C; k++) v += part[((prt * C + k) * 16u + row % 16u) * (TOK + 1u) + tok];
-            epi.put(out, out_dim, t0 + tok, r0 + row, v, bias, res);
+            epi.put(out, out_dim, t0 + tok, r0 + row, v, term);
         }
     }
 }

@@ -4,11 +4,9 @@
 //   FusedOut: out[t][r] = act(v + bias[r]) + residual[t][r], rows of both
 //             arrays at a stride of their own
 //
-// What an epilogue adds is fetched (bias, residual) before the sum it belongs to
-// is complete, so that its loads run beside the weights'; put finishes the sum.
-// What a call leaves out is read from a spare address, at offset 0, and not
-// used: no branch around a load, which would make the compiler wait for every
-// load before it.
+// What an epilogue adds (Term) is fetched ahead of the sum it belongs to, and ahead
+// of the loads that the sum waits for: behind a branch that leaves a fetch out, the
+// compiler can only count what was requested after it.
 #pragma once
 
 #include "pk_common.h"
@@ -20,7 +18,7 @@ namespace pk {
 // that far from 0 the error does not grow with x as exp2(x log2(e)) alone would;
 // 2^lo = 1 + lo ln 2. lo is bounded where p is past exp2's range.
 PK_DEV float exp_near(float x) {
-    constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f;
+    constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
     const float p = x * kHi;
     const float lo = __builtin_fmaf(x, kLo, __builtin_fmaf(x, kHi, -p));
     return __builtin_amdgcn_exp2f(p) *
@@ -29,37 +27,53 @@ PK_DEV float exp_near(float x) {
 PK_DEV float sigmoid_near(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_near(-x)); }
 
 struct PlainOut {
-    PK_DEV float bias_of(uint32_t) const { return 0.0f; }
-    PK_DEV float residual_of(uint32_t, uint32_t) const { return 0.0f; }
-    PK_DEV void put(float *out, uint32_t out_dim, uint32_t t, uint32_t row, float v, float, float) const {
+    struct Term {};
+    PK_DEV Term fetch(uint32_t, uint32_t) const { return {}; }
+    PK_DEV void put(float *out, uint32_t out_dim, uint32_t t, uint32_t row, float v, Term) const {
         out[(uint64_t)t * out_dim + row] = v;
     }
 };
 
 struct FusedOut {
-    const float *bias, *residual;  // a spare address where left out
+    const float *bias, *residual;  // NULL: none
     uint64_t out_stride, res_stride;
     uint32_t act;
-    uint32_t with_bias, with_residual;  // 1 or 0
 
-    PK_DEV float bias_of(uint32_t row) const {
-        return __uint_as_float(ldw32((const uint8_t *)(bias + with_bias * row)));
+    struct Term {
+        float b, r;
+    };
+    PK_DEV Term fetch(uint32_t t, uint32_t row) const {  // an element inside the matrix
+        Term g = {0.0f, 0.0f};
+        if (bias) g.b = bias[row];
+        if (residual) g.r = residual[t * res_stride + row];
+        return g;
     }
-    PK_DEV float residual_of(uint32_t t, uint32_t row) const {
-        return __uint_as_float(ldw32((const uint8_t *)(residual + with_residual * (t * res_stride + row))));
+    PK_DEV void put(float *out, uint32_t, uint32_t t, uint32_t row, float v, Term g) const {
+        float y[1] = {bias ? v + g.b : v};
+        activate(y);
+        out[t * out_stride + row] = residual ? y[0] + g.r : y[0];
     }
-    PK_DEV void put(float *out, uint32_t, uint32_t t, uint32_t row, float v, float b, float r) const {
-        v = activate(v + (with_bias ? b : 0.0f));
-        out[t * out_stride + row] = with_residual ? v + r : v;
-    }
-    PK_DEV float activate(float v) const {
+    // N values at once: one choice of the activation for all
+    template <uint32_t N>
+    PK_DEV void activate(float (&v)[N]) const {
         switch (act) {
-        case PULSAR_EPI_NONE: return v;
-        case PULSAR_EPI_SILU: return v * sigmoid_near(v);
+        case PULSAR_EPI_NONE: break;
+        case PULSAR_EPI_SILU:
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) v[i] *= sigmoid_near(v[i]);
+            break;
         case PULSAR_EPI_GELU:  // v/2 (1 + tanh z) = v / (1 + exp(-2 z)), 2 z = sqrt(8 / pi) (v + 0.044715 v^3)
-            return v * sigmoid_near(1.5957691216057308f * (v + 0.044715f * v * v * v));
-        case PULSAR_EPI_RELU: return v > 0.0f ? v : v != v ? v : 0.0f;
-        default: return sigmoid_near(v);  // PULSAR_EPI_SIGMOID
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++)
+                v[i] *= sigmoid_near(1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
+            break;
+        case PULSAR_EPI_RELU:
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // NaN stays
+            break;
+        default:  // PULSAR_EPI_SIGMOID
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) v[i] = sigmoid_near(v[i]);
         }
     }
 };

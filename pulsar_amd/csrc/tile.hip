@@ -13,6 +13,81 @@
 
 namespace pk {
 
+// The finished sums of a tile: element r of slice n is token t0 + 16 n + 4 q + r,
+// row tile 0 row `row`, row tile 1 16 rows on.
+template <typename T, uint32_t NS>
+PK_DEV void store_tile(const T &tile, const PlainOut &, float *out, uint32_t row, uint32_t out_dim, uint32_t t0,
+                       uint32_t np, uint32_t wk) {
+    const uint32_t q = (threadIdx.x & 63u) >> 4;
+#pragma unroll
+    for (uint32_t n = 0; n < NS; n++)
+#pragma unroll
+        for (uint32_t r = 0; r < 4; r++) {
+            const uint32_t t = 16u * n + 4u * q + r;
+            if (!T::mine(n, r, wk) || t >= np) continue;
+            float *o = out + (uint64_t)(t0 + t) * out_dim + row;
+            if (row < out_dim) o[0] = tile.acc[n][0][r];
+            if (row + 16u < out_dim) o[16] = tile.acc[n][1][r];
+        }
+}
+
+// The same through the epilogue, 8 elements at a time.
+template <typename T, uint32_t NS>
+PK_DEV void store_tile(const T &tile, const FusedOut &e, float *out, uint32_t row, uint32_t out_dim, uint32_t t0,
+                       uint32_t np, uint32_t wk) {
+    // nothing of it is formed before here: the tile has no registers for it
+    asm volatile("" : "+v"(row) : : "memory");
+    const uint32_t q = (threadIdx.x & 63u) >> 4;
+    const bool in0 = row < out_dim, in1 = row + 16u < out_dim;
+    const bool whole = np == T::kTok && __all(in1);  // uniform: no store to leave out
+    const uint32_t r0 = in0 ? row : out_dim - 1u, r1 = in1 ? row + 16u : out_dim - 1u;
+    const float b0 = e.bias ? e.bias[r0] : 0.0f, b1 = e.bias ? e.bias[r1] : 0.0f;
+#pragma unroll
+    for (uint32_t n = 0; n < NS; n++) {
+        bool any = false;
+#pragma unroll
+        for (uint32_t r = 0; r < 4; r++) any |= T::mine(n, r, wk);
+        if (!any) continue;  // uniform
+        float v[8], res[8];
+#pragma unroll
+        for (uint32_t r = 0; r < 4; r++) {
+            v[2 * r] = tile.acc[n][0][r];
+            v[2 * r + 1] = tile.acc[n][1][r];
+        }
+        if (e.residual) {
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++) {
+                const uint32_t t = 16u * n + 4u * q + r, tc = t < np ? t : np - 1u;
+                const float *p = e.residual + (t0 + tc) * e.res_stride;
+                res[2 * r] = p[r0];
+                res[2 * r + 1] = p[r1];
+            }
+        }
+        if (e.bias) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) v[i] += i % 2u ? b1 : b0;
+        }
+        e.activate(v);
+        if (e.residual) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) v[i] += res[i];
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < 4; r++) {
+            const uint32_t t = 16u * n + 4u * q + r;
+            if (!T::mine(n, r, wk)) continue;
+            float *o = out + (t0 + t) * e.out_stride + row;
+            if (whole) {
+                o[0] = v[2 * r];
+                o[16] = v[2 * r + 1];
+            } else if (t < np) {
+                if (in0) o[0] = v[2 * r];
+                if (in1) o[16] = v[2 * r + 1];
+            }
+        }
+    }
+}
+
 // Block = 32 WR weight rows x 16 NS tokens. Blocks go to the 8 XCDs round-
 // robin, each with its own L2: XCD x takes the x-th eighth of the (row block,
 // token tile) items, token tiles fastest, so a row block's weights are read
@@ -30,34 +105,13 @@ __global__ __launch_bounds__(256, 2) void tile_gemm_kernel(float *__restrict__ o
     if (item >= n_item) return;  // block-uniform
     const uint32_t t0 = (item % n_tt) * T::kTok;
     const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, wave = threadIdx.x >> 6;
-    uint32_t row = (item / n_tt * WR + wave % WR) * 32u + (lane & 15u);
+    const uint32_t row = (item / n_tt * WR + wave % WR) * 32u + (lane & 15u);
     const uint32_t np = n_tok - t0 < T::kTok ? n_tok - t0 : T::kTok;
     auto wrow = [&](uint32_t r) { return w + (uint64_t)(r < out_dim ? r : out_dim - 1u) * row_bytes; };
     T tile;
     tile.run(buf0, buf1, lut, wrow(row), wrow(row + 16u), nb, np, (const uint8_t *)(xq + (uint64_t)t0 * nb),
              [&](uint32_t t) { return t * (nb * 292u); });
-    // nothing of the epilogue is fetched or formed before here: the tile has no registers for it
-    asm volatile("" : "+v"(row) : : "memory");
-    const uint32_t at[2] = {row < out_dim ? row : out_dim - 1u, row + 16u < out_dim ? row + 16u : out_dim - 1u};
-    const float bias[2] = {epi.bias_of(at[0]), epi.bias_of(at[1])};
-#pragma unroll
-    for (uint32_t n = 0; n < NS; n++) {
-        float res[4][2];
-#pragma unroll
-        for (uint32_t r = 0; r < 4; r++)
-            if (T::mine(n, r, wave / WR)) {
-                const uint32_t t = 16u * n + 4u * q + r, tc = t0 + (t < np ? t : np - 1u);
-                res[r][0] = epi.residual_of(tc, at[0]);
-                res[r][1] = epi.residual_of(tc, at[1]);
-            }
-#pragma unroll
-        for (uint32_t r = 0; r < 4; r++) {
-            const uint32_t t = 16u * n + 4u * q + r;
-            if (!T::mine(n, r, wave / WR) || t >= np) continue;
-            if (row < out_dim) epi.put(out, out_dim, t0 + t, row, tile.acc[n][0][r], bias[0], res[r][0]);
-            if (row + 16u < out_dim) epi.put(out, out_dim, t0 + t, row + 16u, tile.acc[n][1][r], bias[1], res[r][1]);
-        }
-    }
+    store_tile<T, NS>(tile, epi, out, row, out_dim, t0, np, wave / WR);
 }
 
 template <uint32_t Q, uint32_t WR, uint32_t WK, uint32_t NS>
