@@ -131,8 +131,9 @@ int pulsar_matmul_kq(void *out, const void *w, const void *xq, uint32_t in_dim,
  * at t * res_stride (0: out_dim, the packed rows; never less than out_dim);
  * floats between the rows are left as they are. residual may be out itself, at
  * the same stride (each element is read before it is written); any other
- * overlap of out with an operand is refused. The dots are pulsar_matmul_kq's,
- * bit for bit, with its formats and limits. */
+ * overlap of out with an operand is refused. Formats and limits are
+ * pulsar_matmul_kq's, and so are the dots, but short chunks run a kernel of their
+ * own, which adds a row's super-blocks in another order. */
 int pulsar_matmul_kq_fused(void *out, const void *w, const void *xq, const void *bias,
                            const void *residual, uint32_t in_dim, uint32_t out_dim,
                            uint32_t n_tok, uint64_t row_bytes, uint32_t quant, uint32_t act,

@@ -5,6 +5,8 @@
 // registers for the whole kernel. Weight loads are 16-byte loads at the
 // formats' native (unaligned) offsets; consecutive lanes read consecutive
 // bytes of a row, so every wave-wide load is one contiguous span.
+#include <type_traits>
+
 #include "pk_epilogue.h"
 #include "pk_rowdot.h"
 
@@ -24,6 +26,11 @@ int launch_tile_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_
 template <typename E>
 int launch_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
                 uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi);
+
+// ksplit.hip: short chunks through pulsar_matmul_kq_fused; -1 likewise
+template <typename E>
+int launch_ksplit(uint32_t quant, float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
+                  uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi);
 
 // Each wave streams row passes pass0, pass0 + n_waves, ...: the row's
 // weight units are requested first, then (once per wave) the token's
@@ -214,6 +221,10 @@ static int dense_product(const char *what, void *out, const void *w, const void 
     float *o = (float *)out;
     const uint8_t *wb = (const uint8_t *)w;
     const pulsar_block_q8_K *x = (const pulsar_block_q8_K *)xq;
+    if constexpr (std::is_same_v<E, FusedOut>) {
+        const int r = launch_ksplit(quant, o, wb, x, in_dim, out_dim, n_tok, row_bytes, epi);
+        if (r >= 0) return r;
+    }
     if (n_tok >= PK_MMQ_MIN_TOK) {
         int r = launch_tile_gemm(quant, o, wb, x, in_dim, out_dim, n_tok, row_bytes, epi);
         if (r < 0) r = launch_gemm(quant, o, wb, x, in_dim, out_dim, n_tok, row_bytes, epi);

@@ -1,6 +1,6 @@
-"""pulsar_matmul_kq_fused: its dots are pulsar_matmul_kq's bit for bit, its
-epilogue is held against 64 bits, at the chunk lengths and row counts where the
-product changes its kernel."""
+"""pulsar_matmul_kq_fused: its dots against the oracle, its epilogue against 64
+bits on those dots, at the chunk lengths and row counts where the product changes
+its kernel."""
 import numpy as np
 import pytest
 import torch
@@ -47,13 +47,40 @@ class Case:
         self.w = synth.quant_matrix(quant, rows, n, rng)
         self.x = oracle.quantize_q8_k(rng.standard_normal((T, n)).astype(np.float32))
         self.dw, self.dx = up(self.w), up(self.x)
-        dots = zeros_f32((T, rows))
-        K.matmul_kq(dots, self.dw, self.dx, n, rows, T, self.rb, quant)
-        self.dots = down(dots)
+        # the bare dots; the epilogue is applied to the same sums
+        self.dots = down(self.run(zeros_f32((T, rows)), None, None, EPI_NONE))
         # bias and residual of the dots' size, so that each term shows
         size = max(float(np.abs(self.dots).mean()), 1e-3)
         self.bias = (size * rng.standard_normal(rows)).astype(np.float32)
         self.res = (size * rng.standard_normal((T, rows))).astype(np.float32)
+
+    def check_dots(self):
+        """The dots against the oracle, a sample of the rows around the tiles'
+        edges and of the tokens: exact integers per super-block on both sides, at
+        most 6 roundings of each product's size where the two products of a format
+        with mins cancel (P, M below), 1e-5 sum |f_b| for the sums' order. Where a
+        super-block is itself a sum of up to 16 f32 terms, of 16 or 32 values each,
+        that may cancel: 2 roundings of each term and 15 additions on either side,
+        34 2^-24 of the terms' sizes."""
+        at = sorted({r for e in (0, 16, 32, 64, 128, self.rows // 2, self.rows) for r in range(e - 2, e + 3)
+                     if 0 <= r < self.rows})
+        tok = sorted({t for e in (0, 16, 32, 48, 64, 128, self.T) for t in range(e - 2, e + 2) if 0 <= t < self.T})
+        w, x = np.ascontiguousarray(self.w[at]), np.ascontiguousarray(self.x[tok])
+        want, scale = oracle.rows_dot(w, self.rb, len(at), x, self.n, len(tok), self.quant, 8)
+        bound = scale
+        if self.quant in (fm.QUANT_Q4_K, fm.QUANT_Q5_K, fm.QUANT_Q2_K):
+            w0, off = w.copy(), 82 if self.quant == fm.QUANT_Q2_K else 2
+            w0.reshape(-1, fm.BLOCK_LAYOUT[self.quant][1])[:, off:off + 2] = 0
+            _, p = oracle.rows_dot(w0, self.rb, len(at), x, self.n, len(tok), self.quant, 8)
+            bound = scale + 6 * 2.0**-24 / 1e-5 * (2 * p + scale)
+        if self.quant in (fm.QUANT_IQ4_NL, fm.QUANT_NVFP4):
+            v = np.stack([oracle.dequant_row(self.quant, r, self.n) for r in w]).astype(np.float64)
+            b = x.reshape(len(tok), -1, 292)
+            y = np.ascontiguousarray(b[..., 4:260]).view(np.int8) * np.ascontiguousarray(b[..., :4]).view(np.float32)
+            terms = np.einsum("tgi,rgi->trg", y.reshape(len(tok), -1, 16).astype(np.float64), v.reshape(len(at), -1, 16))
+            bound = bound + 34 * 2.0**-24 / 1e-5 * np.abs(terms).sum(-1).reshape(bound.shape)
+        assert_rows_close(self.dots[np.ix_(tok, at)], want.reshape(len(tok), len(at)),
+                          bound.reshape(len(tok), len(at)), (self.quant, self.rows, self.n, self.T))
 
     def run(self, out, bias, res, act, **kw):
         K.matmul_kq_fused(out, self.dw, self.dx, bias, res, self.n, self.rows, self.T, self.rb, self.quant, act, **kw)
@@ -61,21 +88,56 @@ class Case:
 
 
 # rows, values, tokens: the lane kernels (1 to 4 tokens, several rows to a wave,
-# rows of more than 8 units a lane), the 16-row kernel (5 to 31), each tile
+# rows of more than 8 units a lane), the 16-row kernel, each wide tile, the K split
+# with every width of its token tile and more and fewer super-blocks than waves
 SHAPES = [(1, 256, 1), (33, 512, 1), (500, 4096, 1), (5000, 256, 1), (65, 33024, 1), (40, 33024, 3), (130, 8448, 2),
-          (70, 16640, 4), (301, 768, 3), (100, 512, 5), (8200, 256, 16), (513, 1024, 31), (4129, 512, 33),
-          (1000, 768, 70), (8300, 256, 130), (4130, 256, 500), (14400, 256, 300)]
+          (70, 16640, 4), (301, 768, 3), (16500, 512, 2), (100, 512, 5), (8200, 256, 16), (16500, 768, 12),
+          (513, 1024, 31), (70, 4352, 14), (4129, 512, 33), (8300, 512, 49), (1000, 768, 70), (1100, 2816, 100),
+          (2049, 2304, 33), (4096, 2048, 31), (1500, 256, 64), (8300, 256, 130), (4130, 256, 500), (14400, 256, 300),
+          (17, 2304, 400)]
 
 
 @pytest.mark.parametrize("quant", fm.DENSE_QUANTS)
 @pytest.mark.parametrize("rows,n,T", SHAPES)
 def test_shapes(dev, quant, rows, n, T):
     c = Case(quant, rows, n, T)
-    bare = down(c.run(zeros_f32((T, rows)), None, None, EPI_NONE))
-    assert np.array_equal(bare.view(np.uint32), c.dots.view(np.uint32))
+    c.check_dots()
     act = ACTS[(rows + T + quant) % 5]
     got = down(c.run(zeros_f32((T, rows)), up_f32(c.bias), up_f32(c.res), act))
     assert_epilogue(got, c.dots, c.bias, act, c.res, (quant, act))
+
+
+@pytest.mark.parametrize("rows,n,T", [(16500, 512, 12), (4130, 256, 500), (14400, 256, 300), (500, 4096, 1)])
+def test_same_kernel_same_bits(dev, rows, n, T):
+    """Where both run the same kernel: pulsar_matmul_kq's dots bit for bit."""
+    c = Case(fm.QUANT_Q4_K, rows, n, T)
+    dots = zeros_f32((T, rows))
+    K.matmul_kq(dots, c.dw, c.dx, n, rows, T, c.rb, c.quant)
+    assert np.array_equal(down(dots).view(np.uint32), c.dots.view(np.uint32))
+
+
+@pytest.mark.parametrize("quant", fm.DENSE_QUANTS)
+@pytest.mark.parametrize("rows,n,T", [(200, 2816, 5), (65, 5120, 40), (129, 256, 64)])
+def test_integer_stage_exact(dev, quant, rows, n, T):
+    """Unit scales and whole q8 values, one super-block's sum at a time: exact."""
+    if quant not in (fm.QUANT_Q4_K, fm.QUANT_Q5_K, fm.QUANT_Q2_K, fm.QUANT_Q6_K, fm.QUANT_Q3_K, fm.QUANT_IQ4_XS):
+        pytest.skip("no whole weight scale")
+    rng = np.random.default_rng(n)
+    w = synth.quant_matrix(quant, rows, n, rng)
+    blk = w.reshape(-1, fm.BLOCK_LAYOUT[quant][1])
+    for off in {fm.QUANT_Q4_K: (0, 2), fm.QUANT_Q5_K: (0, 2), fm.QUANT_Q2_K: (80, 82), fm.QUANT_Q6_K: (208,),
+                fm.QUANT_Q3_K: (108,), fm.QUANT_IQ4_XS: (0,)}[quant]:
+        blk[:, off], blk[:, off + 1] = 0x00, 0x3C  # 1.0
+    qs = rng.integers(-9, 10, (T, n // 256, 256)).astype(np.int8)  # sums stay below 2^24
+    x = np.zeros((T, n // 256, 292), np.uint8)
+    x[..., 0:4] = np.array([1.0], np.float32).view(np.uint8)
+    x[..., 4:260] = qs.view(np.uint8)
+    x[..., 260:] = qs.reshape(T, -1, 16, 16).astype(np.int16).sum(-1).astype(np.int16).view(np.uint8).reshape(T, -1, 32)
+    x = x.reshape(T, -1)
+    out = zeros_f32((T, rows))
+    K.matmul_kq_fused(out, up(w), up(x), None, None, n, rows, T, row_bytes(quant, n), quant, EPI_NONE)
+    want, _ = oracle.rows_dot(w, row_bytes(quant, n), rows, x, n, T, quant, 8)
+    assert np.array_equal(down(out), want.reshape(T, rows))
 
 
 @pytest.mark.parametrize("T", [1, 3, 9, 33, 260])
