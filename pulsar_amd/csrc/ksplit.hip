@@ -150,18 +150,35 @@ static int launch_ksplit_n(float *out, const uint8_t *w, const pulsar_block_q8_K
     return launch_ok("matmul_kq_fused K split launch");
 }
 
+static uint64_t ksplit_tiles(uint32_t out_dim, uint32_t n_tok) {  // of 16 rows x 16 tokens
+    return (uint64_t)((n_tok + 15u) / 16u) * ((out_dim + 15u) / 16u);
+}
+
+// The token tile with the shortest time, which goes by the rounds its blocks take:
+// a CU holds two blocks of one slice at once, one of more (registers). Time of a
+// round as measured, in hundredths of one of two slices (Q4_K 4096 x 4096: 4.9 us).
+struct KPlan {
+    uint32_t ns;
+    uint64_t cost;
+};
+static KPlan ksplit_plan(uint32_t out_dim, uint32_t n_tok) {
+    const uint64_t slices = (n_tok + 15u) / 16u, row_tiles = (out_dim + 15u) / 16u;
+    KPlan best = {1u, slices * row_tiles <= 256u ? 70u : (slices * row_tiles + 511u) / 512u * 106u};
+    const uint64_t round[3] = {100u, 140u, 162u};
+    for (uint32_t ns = 2; ns <= 4u && ns <= slices; ns++) {
+        const uint64_t cost = ((slices + ns - 1u) / ns * row_tiles + 255u) / 256u * round[ns - 2u];
+        if (cost <= best.cost) best = {ns, cost};
+    }
+    return best;
+}
+
 template <uint32_t Q, typename E>
 static int launch_ksplit_q(float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t nb, uint32_t out_dim,
                            uint32_t n_tok, uint64_t row_bytes, const E &epi) {
-    // The widest token tile (a row is decoded once per tile) that leaves a block
-    // for every CU, and no wider than it takes for as many tiles
-    const uint32_t slices = (n_tok + 15u) / 16u, row_tiles = (out_dim + 15u) / 16u;
-    uint32_t ns = slices < 4u ? slices : 4u;
-    while (ns > 1u && (uint64_t)((slices + ns - 1u) / ns) * row_tiles < 256u) ns--;
-    const uint32_t tiles = (slices + ns - 1u) / ns;
-    ns = (slices + tiles - 1u) / tiles;
+    const uint32_t ns = ksplit_plan(out_dim, n_tok).ns;
+    const uint64_t tiles = ksplit_tiles(out_dim, n_tok);
 #define PK_KS(NS, W) return launch_ksplit_n<Q, NS, W>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi)
-    if (ns == 1u && nb >= 16u && (uint64_t)slices * row_tiles <= 128u) PK_KS(1, 16);
+    if (ns == 1u && nb >= 16u && tiles <= 128u) PK_KS(1, 16);
     if (ns == 1u) PK_KS(1, 8);
     if (ns == 2u) PK_KS(2, 8);
     if (ns == 3u) PK_KS(3, 8);
@@ -169,37 +186,35 @@ static int launch_ksplit_q(float *out, const uint8_t *w, const pulsar_block_q8_K
 #undef PK_KS
 }
 
-// Where this kernel was the faster one, by tiles of 16 rows x 16 tokens (weights
-// from HBM, both sides timed: 43879 shapes of 48 to 16384 rows, 1 to 56 super-
-// blocks, 2 to 500 tokens, 7 formats; where it runs it is 1.4 times as fast on
-// average). Above `most` tiles the wide tile or, up to 16 tokens, the 16-row kernel
-// has the whole chip at work too, and shares a decoded row among more tokens (Q4_K
-// 4096 x 4096: 33 tokens 8.5 against 11.0 us, 100 tokens 18.9 against 15.2). Below
-// `least`, for long rows, the blocks leave most CUs idle, and kernels that spread
-// rows further are ahead: the lane kernels, a wave per row (Q3_K 83 x 12032, 2
-// tokens: 14.7 against 4.4 us; 4096 x 4096, 4 tokens, Q4_K: 5.0 against 8.2), and
-// for Q6_K, whose decode is the longest, the 16-row kernel.
+// Where this kernel was the faster one (weights from HBM, both sides timed: 97442
+// shapes of 48 to 16384 rows, 1 to 56 super-blocks, 2 to 500 tokens, 7 formats).
+// It is ahead as long as its blocks take few rounds, more for formats of a longer
+// decode (`most`, in the plan's cost): then the wide tile or, up to 16 tokens, the
+// 16-row kernel has the whole chip at work too and shares a decoded row among more
+// tokens (Q4_K 4096 x 4096: 33 tokens 8.5 against 11.0 us, 100 tokens 18.9 against
+// 15.2). Below `least` tiles of long rows its blocks leave most CUs idle, and
+// kernels that spread rows further are ahead: the lane kernels, a wave per row
+// (Q3_K 83 x 12032, 2 tokens: 14.7 against 4.4 us; Q4_K 4096 x 4096, 4 tokens: 5.0
+// against 8.2), and for Q6_K, whose decode is the longest, the 16-row kernel.
 static bool ksplit_wins(uint32_t quant, uint32_t nb, uint32_t out_dim, uint32_t n_tok) {
-    const uint64_t tiles = (uint64_t)((n_tok + 15u) / 16u) * ((out_dim + 15u) / 16u);
+    if (n_tok == 1u) return false;
+    const uint64_t tiles = ksplit_tiles(out_dim, n_tok);
     const bool q45 = quant == PULSAR_QUANT_Q4_K || quant == PULSAR_QUANT_Q5_K, q2 = quant == PULSAR_QUANT_Q2_K;
     const bool q6 = quant == PULSAR_QUANT_Q6_K, iq = quant == PULSAR_QUANT_IQ4_XS || quant == PULSAR_QUANT_IQ2_XXS;
-    uint32_t least = 0u, most;
-    if (n_tok == 1u) return false;
-    if (n_tok == 2u) {
-        if (q6 && nb > 8u) return false;
-        least = q45 || q2 ? 65u : 129u;
-        most = iq ? 512u : 1024u;
-    } else if (n_tok <= 4u) {
-        least = q6 ? 129u : 65u;
-        most = 1024u;
+    uint32_t least = 0u, most = 212u;
+    if (n_tok <= 4u) {
+        if (q6 && nb > 8u && (n_tok == 2u || (nb <= 16u && tiles > 256u))) return false;
+        if (iq && n_tok == 2u) most = 106u;
+        least = q6 || (n_tok == 2u && !q45 && !q2) ? 129u : 65u;
     } else if (n_tok <= 32u) {
         if (q6 && nb > 32u && n_tok <= 16u) return false;
         least = q45 || (q6 && nb <= 16u) ? 0u : q6 ? (nb <= 32u ? 257u : 513u) : 33u;
-        most = n_tok <= 16u ? 1024u : q2 ? 512u : q45 || quant == PULSAR_QUANT_IQ2_XXS ? 1024u : 1536u;
+        if (n_tok > 16u && (q6 || quant == PULSAR_QUANT_Q3_K)) most = 300u;
     } else {
-        most = n_tok > 64u || q45 || q2 ? 512u : 2048u;
+        least = n_tok > 64u || q45 || q6 ? 0u : 17u;
+        most = q6 || iq || quant == PULSAR_QUANT_Q3_K ? 300u : n_tok > 128u && !q45 ? 162u : 212u;
     }
-    return tiles <= most && (nb <= 8u || tiles >= least);
+    return ksplit_plan(out_dim, n_tok).cost <= most && (nb <= 8u || tiles >= least);
 }
 
 // -1: no such kernel for the format, or another one is as fast
