@@ -236,7 +236,7 @@ int pulsar_router_select(void *selected, void *weights, const void *logits,
  *     all 0 where every winner's s is 0 in 64 bits); times weight_scale
  * Ids are decided as c stands in 64 bits, whatever f32 would round it to.
  * n_expert <= 1024, a multiple of n_group <= 64; k_used <= 64 and <= the
- * experts of topk_group groups. */
+ * experts of topk_group groups; n_tok <= 2^25. */
 int pulsar_router_select_groups(void *selected, void *weights, const void *logits,
                                 const void *bias, uint32_t n_expert, uint32_t k_used,
                                 uint32_t n_group, uint32_t topk_group, uint32_t group_top,
@@ -311,8 +311,10 @@ int pulsar_moe_group_csr(void *gptrs, void *starts, void *pairs, const void *ptr
  * [n_tok][k_used]; ids outside [0, n_expert) get no pair, so the caller zeroes
  * partial as for any CSR. slot_weights f32 [n_tok][k_used + n_shared], left out
  * where NULL: router_weights [n_tok][k_used], then 1 for the shared slots.
- * n_expert <= 1024, k_used + n_shared <= 16, n_shared <= 4, n_tok <= 2^28, n_tok * (k_used +
- * n_shared) < 2^31; bank and shared are host pointers read at launch. */
+ * n_expert <= 1024, k_used + n_shared <= 16, n_shared <= 4, n_tok <= 2^28,
+ * n_tok * (k_used + n_shared) < 2^31; bank and shared are host pointers read at
+ * launch. gptrs and starts are working memory too while the call runs: two
+ * calls that may run at once take buffers of their own. */
 int pulsar_moe_group_ids(void *gptrs, void *starts, void *pairs, void *slot_weights,
                          const void *selected, const void *router_weights,
                          const pulsar_expert_bank *bank, uint32_t n_expert,

@@ -14,11 +14,8 @@
 
 namespace pk {
 
-#ifndef PK_RG_MANY
-#define PK_RG_MANY 4096u
-#endif
-
 constexpr uint32_t kMaxGroups = 64;
+constexpr uint32_t kMaxTokens = 1u << 25;  // a launch has below 2^32 threads, 64 a token at most
 
 struct GroupRoute {
     const float *logits, *bias;
@@ -490,7 +487,8 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint
     // take anyway (p + b, whose sum is f32's, by the keys alone)
     won = kk == r.k_used ? next : won;
     const bool here = kk < r.k_used, seen = kk <= r.k_used;
-    const uint32_t id = seen ? (15u - (won >> 5 & 15u)) * per_lane + 31u - (won & 31u) : 0u;
+    // (a key of 0, no expert's, stands for one as well: such a row is unsure)
+    const uint32_t id = seen ? min_u((15u - (won >> 5 & 15u)) * per_lane + 31u - (won & 31u), E - 1u) : 0u;
     const double raw = (double)row_l[place(id)];
     double w;
     if (r.softmax) {
@@ -536,7 +534,7 @@ extern "C" int pulsar_router_select_groups(void *selected, void *weights, const 
                                            uint32_t n_expert, uint32_t k_used, uint32_t n_group, uint32_t topk_group,
                                            uint32_t group_top, uint32_t score, uint32_t renorm, float weight_scale,
                                            uint32_t n_tok) {
-    if (!selected || !weights || !logits || n_tok == 0 || n_expert == 0 || n_expert > 64u * pk::kMaxPerLane ||
+    if (!selected || !weights || !logits || n_tok == 0 || n_tok > pk::kMaxTokens || n_expert == 0 || n_expert > 64u * pk::kMaxPerLane ||
         n_group == 0 || n_group > pk::kMaxGroups || n_expert % n_group != 0 || topk_group == 0 ||
         topk_group > n_group || group_top == 0 || group_top > 2u || k_used == 0 || k_used > 64u ||
         k_used > n_expert / n_group * topk_group || score > 1u)
@@ -546,7 +544,7 @@ extern "C" int pulsar_router_select_groups(void *selected, void *weights, const 
     // whole lanes of the 16 a token has: the f32 kernel
     if (n_expert <= 512u && k_used <= 16u && 16u % n_group == 0u && (n_group == 1u || n_expert % 16u == 0u)) {
         const uint32_t per_lane = (n_expert + 15u) / 16u;
-        const bool many = n_tok >= PK_RG_MANY;
+        const bool many = n_tok >= 4096u;
 #define PK_RGFK(J, K, W)                                                                                       \
     hipLaunchKernelGGL((pk::route_groups_kernel<J, K, W>), dim3((n_tok + 4u * W - 1u) / (4u * W)), dim3(64u * W), 0, \
                        pk::stream(), r, per_lane)

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256, 2) void tile_gemm_kernel(float *__restrict__ o
     const uint32_t item = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     if (item >= n_item) return;  // block-uniform
     const uint32_t t0 = (item % n_tt) * T::kTok;
-    const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t row = (item / n_tt * WR + wave % WR) * 32u + (lane & 15u);
     const uint32_t np = n_tok - t0 < T::kTok ? n_tok - t0 : T::kTok;
     auto wrow = [&](uint32_t r) { return w + (uint64_t)(r < out_dim ? r : out_dim - 1u) * row_bytes; };

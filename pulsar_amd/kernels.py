@@ -16,7 +16,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from .formats import EXPERT_PTRS_BYTES
+from .formats import BLOCK_LAYOUT, EXPERT_PTRS_BYTES
 
 
 class KernelError(RuntimeError):
@@ -59,7 +59,7 @@ def _room(buf, nbytes: int, op: str, what: str, device: int) -> int:
     """The device address of `buf`, which the launch uses the first nbytes
     bytes of; a tensor has to be contiguous, that large and on the current
     device (a raw address is the caller's word for all three)."""
-    if buf is None or not hasattr(buf, "data_ptr"):
+    if buf is None or type(buf) is int:
         return _ptr(buf)
     if buf.get_device() != device:
         _misplaced(buf, op, what)
@@ -83,7 +83,7 @@ def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str, device: i
     """The device address of n_rows rows of dim floats, `stride` floats apart.
     A tensor may be a view of columns of a wider array: it has to be f32 [..,
     dim] with that stride, or contiguous and large enough."""
-    if buf is None or not hasattr(buf, "data_ptr"):
+    if buf is None or type(buf) is int:
         return _ptr(buf)
     if buf.get_device() != device:
         _misplaced(buf, op, what)
@@ -105,10 +105,12 @@ def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok
     bias) + residual[t] (formats.EPI_* codes; bias and residual may be None).
     Strides in floats, 0 for packed rows; residual may be out itself."""
     op, dev = "matmul_kq_fused", _device()
+    block, block_bytes = BLOCK_LAYOUT.get(quant, (1, 0))
+    w_bytes = (out_dim - 1) * row_bytes + in_dim // block * block_bytes
     xq_bytes, so, sr = n_tok * -(-in_dim // 256) * 292, out_stride or out_dim, res_stride or out_dim
     _check(
         _lib.load().pulsar_matmul_kq_fused(
-            _rows(out, n_tok, out_dim, so, op, "out", dev), _room(w, (out_dim - 1) * row_bytes, op, "w", dev),
+            _rows(out, n_tok, out_dim, so, op, "out", dev), _room(w, w_bytes, op, "w", dev),
             _room(xq, xq_bytes, op, "xq", dev), _room(bias, 4 * out_dim, op, "bias", dev),
             _rows(residual, n_tok, out_dim, sr, op, "residual", dev), in_dim, out_dim, n_tok, row_bytes, quant, act,
             out_stride, res_stride),

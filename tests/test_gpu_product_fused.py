@@ -261,3 +261,6 @@ def test_wrapper_refuses_short_tensors(dev):
             c.run(out, bias, res, EPI_NONE)
     with pytest.raises(ValueError, match="f32"):
         c.run(z.double(), None, None, EPI_NONE)
+    c.dw = c.dw.reshape(-1)[:-1]  # the last row, but for a byte
+    with pytest.raises(ValueError, match="w has to"):
+        c.run(z, None, None, EPI_NONE)

@@ -24,7 +24,7 @@ ROUTE = dict(selected=A[0], weights=A[1], logits=A[2], bias=A[3], n_expert=32, k
 
 
 @pytest.mark.parametrize("change", [
-    dict(selected=0), dict(weights=0), dict(logits=0), dict(n_tok=0), dict(n_expert=0), dict(n_expert=1032),
+    dict(selected=0), dict(weights=0), dict(logits=0), dict(n_tok=0), dict(n_tok=2**25 + 1), dict(n_expert=0), dict(n_expert=1032),
     dict(n_group=0), dict(n_group=5), dict(n_group=128, n_expert=1024), dict(topk_group=0), dict(topk_group=9),
     dict(group_top=0), dict(group_top=3), dict(k_used=0), dict(k_used=9), dict(k_used=65, n_expert=512, topk_group=8),
     dict(score=2)])
