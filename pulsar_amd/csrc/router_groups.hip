@@ -191,18 +191,19 @@ __global__ __launch_bounds__(256) void route_groups_f64_kernel(GroupRoute r) {
 
 // ---- four tokens a wave, in f32 with a proof of the order -----------------
 //
-// 16 lanes a token (a DPP row, so that every exchange is a DPP move), lane kk
-// holds experts kk Jr .. kk Jr + Jr - 1. The choice c is taken in f32 and scaled
+// 16 lanes a token (a DPP row, so that every exchange is a DPP move). A group has
+// `of` of them (a power of two), each per_lane of its experts in their order, so
+// a lower (lane, place) is a lower id. The choice c is taken in f32 and scaled
 // to a 23-bit integer q over a window below the row's best; q, the lane and the
 // expert's place in it make one unique 32-bit key, so that sorting keys is
 // single max / min operations. The error of q is bounded (err), so keys whose q
 // lie `gap` apart are in the order of the 64-bit scores. That settles which
-// experts win; the winners, and the one behind them if it is close, are then put
-// to the test by their 64-bit scores. A row that fails it (ties, an order that
-// f32 swapped), whose groups at the border lie closer than the gap, that has
+// groups stay, but for a row with two at the border closer than that, whose
+// groups' best are scored in 64 bits, and which experts win; the winners, and the
+// one behind them if it is close, are then put to the test by their 64-bit
+// scores. A row that fails one (ties, an order that f32 swapped), that has
 // infinite scores or runs out of candidates or of the window, is done again by
-// route_token_f64: of a trained router's rows one in some thousands, rows of ties
-// always.
+// route_token_f64: rows of ties always, a trained router's hardly ever.
 
 constexpr uint32_t kQShift = 9;  // below q: 15 - kk in 4 bits, 31 - j in 5
 constexpr float kSteps = 8384000.0f;  // q < 2^23, with room for 4600 steps of rounding
@@ -273,42 +274,70 @@ PK_DEV T row_reduce(T v, F f) {
 PK_DEV float row_max_f(float v) {
     return row_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
-PK_DEV double row_sum(double v) {
+template <typename F>
+PK_DEV double halves(double v, F f) {  // f of both words
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)f((uint32_t)(u >> 32)) << 32 | f((uint32_t)u));
+}
+PK_DEV double partner_f64(double v, uint32_t m) {
+    return halves(v, [m](uint32_t h) { return (uint32_t)partner((int32_t)h, m); });
+}
+template <typename F>
+PK_DEV double row_reduce_f64(double v, F f) {
 #pragma unroll
-    for (uint32_t m = 1; m < 16; m <<= 1) {
-        uint64_t u = __builtin_bit_cast(uint64_t, v);
-        const uint32_t lo = (uint32_t)partner((int32_t)(uint32_t)u, m), hi = (uint32_t)partner((int32_t)(u >> 32), m);
-        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-    }
+    for (uint32_t m = 1; m < 16; m <<= 1) v = f(v, partner_f64(v, m));
     return v;
+}
+PK_DEV double row_sum(double v) {
+    return row_reduce_f64(v, [](double a, double b) { return a + b; });
 }
 // lane i gets lane i + 1 of its row
 PK_DEV double row_behind(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x101, 0xF, 0xF, true);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), 0x101, 0xF, 0xF, true);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    return halves(v, [](uint32_t h) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)h, 0x101, 0xF, 0xF, true);
+    });
 }
 // lane i gets lane (i - N) % 16 of its row
 template <uint32_t N>
 PK_DEV uint32_t row_turn(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xF, 0xF, false);
 }
+template <uint32_t N>
+PK_DEV double row_turn(double v) {
+    return halves(v, [](uint32_t h) { return row_turn<N>(h); });
+}
 // how many of the row's other groups, of G lanes each, have a larger v
-template <uint32_t G, uint32_t N = G>
-PK_DEV uint32_t groups_ahead(uint32_t v) {
+template <uint32_t G, uint32_t N = G, typename T>
+PK_DEV uint32_t groups_ahead_of(T v) {
     if constexpr (N >= 16u)
         return 0u;
     else
-        return (row_turn<N>(v) > v ? 1u : 0u) + groups_ahead<G, N + G>(v);
+        return (row_turn<N>(v) > v ? 1u : 0u) + groups_ahead_of<G, N + G>(v);
+}
+template <typename T>
+PK_DEV uint32_t groups_ahead(T v, uint32_t of) {  // `of` is uniform
+    return of == 1u   ? groups_ahead_of<1>(v)
+           : of == 2u ? groups_ahead_of<2>(v)
+           : of == 4u ? groups_ahead_of<4>(v)
+                      : groups_ahead_of<8>(v);
 }
 
-// J: experts a lane, 16 J >= n_expert; K: k_used <= K. Groups are whole lanes:
-// n_group divides 16, and 16 n_expert where there are several.
+struct GroupLanes {
+    uint32_t size, of_log2, of, per_lane;  // experts and lanes of a group, experts of a lane
+    uint32_t by_size, by_lane;  // 2^20 / size and / per_lane, rounded up
+
+    // where a row of `pitch` floats a lane has expert e; e < 512, so the quotients are exact
+    PK_DEV uint32_t at(uint32_t e, uint32_t pitch) const {
+        const uint32_t g = e * by_size >> 20, i = e - g * size, l = i * by_lane >> 20;
+        return (g * of + l) * pitch + i - l * per_lane;
+    }
+};
+
+// J: experts a lane has room for; K: k_used <= K. n_group <= 16.
 // W: waves of a block (blocks start at about one in 4 ns, so a long chunk takes
 // few large ones).
 template <uint32_t J, uint32_t K, uint32_t W>
-__global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint32_t per_lane) {
+__global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, GroupLanes g) {
     constexpr uint32_t kJ64 = J < 4u ? 1u : J / 4u;
     // A lane's experts in LDS: rows are read from memory as they lie, 16 lanes
     // that read J floats each then find them on distinct banks
@@ -318,13 +347,8 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint
     __shared__ __align__(16) float bias_l[kRow];
     const uint32_t lane = threadIdx.x & 63u, kk = lane & 15u, E = r.n_expert;
     const uint32_t token0 = (blockIdx.x * W + (threadIdx.x >> 6)) * 4u;
-    const uint32_t part = 65536u / per_lane + 1u;  // e / per_lane = e part >> 16 for e < 1024
-    auto place = [&](uint32_t e) {
-        const uint32_t o = e * part >> 16;
-        return o * kPitch + (e - o * per_lane);
-    };
     float *mine_l = rows_l[threadIdx.x >> 6];
-    if (J >= 4u && E == 16u * J) {  // rows of whole 16-byte pieces, one after the other
+    if (J >= 4u && E == 16u * J && g.of * r.n_group == 16u) {  // rows of whole 16-byte pieces, one after the other
 #pragma unroll
         for (uint32_t i = 0; i < J / 4u; i++) {
             const uint32_t f = (lane + 64u * i) * 4u, t = f / (16u * J), e = f % (16u * J);
@@ -335,13 +359,17 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint
     } else {
         for (uint32_t i = lane; i < 4u * kRow; i += 64u) mine_l[i] = __builtin_nanf("");  // no expert there
         __builtin_amdgcn_wave_barrier();  // a wave's LDS writes land in order
-        for (uint32_t t = 0; t < 4u; t++) {
-            const uint32_t token = token0 + t < r.n_tok ? token0 + t : r.n_tok - 1u;
-            for (uint32_t e = lane; e < E; e += 64u) mine_l[t * kRow + place(e)] = r.logits[(uint64_t)token * E + e];
+        for (uint32_t e = lane; e < E; e += 64u) {
+            const uint32_t at = g.at(e, kPitch);
+#pragma unroll
+            for (uint32_t t = 0; t < 4u; t++) {
+                const uint32_t token = token0 + t < r.n_tok ? token0 + t : r.n_tok - 1u;
+                mine_l[t * kRow + at] = r.logits[(uint64_t)token * E + e];
+            }
         }
     }
     if (r.bias)
-        for (uint32_t e = threadIdx.x; e < E; e += 64u * W) bias_l[place(e)] = r.bias[e];
+        for (uint32_t e = threadIdx.x; e < E; e += 64u * W) bias_l[g.at(e, kPitch)] = r.bias[e];
     __syncthreads();
     if (token0 >= r.n_tok) return;  // whole wave, behind the block's only barrier
     const uint32_t token = token0 + (lane >> 4);
@@ -404,6 +432,17 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint
 #pragma unroll
         for (uint32_t j = 0; j < J; j++) c[j] += bias_l[kk * kPitch + j];
     }
+    // The score in 64 bits of the expert at `at` of the row, a softmax's without
+    // its sum; the choice of it, a softmax's but for z's error, at most zerr of the
+    // score (as f32's above: 20.7 + 9 steps)
+    constexpr double zerr = 33.0 * 0x1p-24;
+    const double rz = r.softmax && !by_logit ? 1.0 / (double)z : 1.0;
+    auto score = [&](uint32_t at) {
+        const double raw = (double)row_l[at];
+        const double e = exp(r.softmax ? raw - (double)m : -fabs(raw));
+        return r.softmax ? e : (raw >= 0.0 ? 1.0 : e) / (1.0 + e);
+    };
+    auto choice = [&](double s, uint32_t at) { return s * rz + (r.bias ? (double)bias_l[at] : 0.0); };
     float hi = -INFINITY;
 #pragma unroll
     for (uint32_t j = 0; j < J; j++) hi = fmaxf(hi, c[j]);
@@ -430,28 +469,63 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint
 #pragma unroll
     for (uint32_t k = 0; k < K; k++) top[k] = k < N ? s[0][k < N ? k : 0u] | (15u - kk) << 5 : 0u;
     if (r.n_group > 1u) {
-        const uint32_t lanes = 16u / r.n_group;  // of a group
         uint32_t g0 = top[0], g1 = K > 1u ? top[K > 1u ? 1 : 0] : 0u;
 #pragma unroll
         for (uint32_t st = 1; st < 16u; st <<= 1)
-            if (st < lanes) {  // uniform
+            if (st < g.of) {  // uniform
                 const uint32_t o0 = (uint32_t)partner((int32_t)g0, st), o1 = (uint32_t)partner((int32_t)g1, st);
                 g1 = max_u(max_u(g1, o1), min_u(g0, o0));
                 g0 = max_u(g0, o0);
             }
         const bool two = r.group_top == 2u && E > r.n_group;  // a group of one expert is that one
         const uint32_t q0 = g0 >> kQShift, q1 = g1 >> kQShift, stand = q0 + (two ? q1 : 0u);
+        const bool real = kk < r.n_group * g.of;
         // a group that stands with one, or with what the window cut, has no sum here
-        unsure |= two && q1 == 0u;
-        const uint32_t ahead = lanes == 2u   ? groups_ahead<2>(stand)
-                               : lanes == 4u ? groups_ahead<4>(stand)
-                               : lanes == 8u ? groups_ahead<8>(stand)
-                                             : groups_ahead<1>(stand);
-        const bool kept = ahead < r.topk_group;
-        const uint64_t all = __ballot(kept);
-        unsure |= (uint32_t)__builtin_popcount((uint32_t)(all >> (lane & 48u)) & 0xffffu) != r.topk_group * lanes;
+        unsure |= real && two && q1 == 0u;
+        bool kept = real && groups_ahead(stand, g.of) < r.topk_group;
         const uint32_t last = row_reduce(kept ? stand : UINT32_MAX, min_u), next = row_reduce(kept ? 0u : stand, max_u);
-        unsure |= r.topk_group < r.n_group && last - next < 2u * gap;
+        auto lanes_of = [&](bool b) {  // lanes of the row that say b
+            return (uint32_t)__builtin_popcount((uint32_t)(__ballot(b) >> (lane & 48u)) & 0xffffu);
+        };
+        const bool doubt = lanes_of(kept) != r.topk_group * g.of ||  // equal ones
+                           (r.topk_group < r.n_group && last < next + 2u * gap);
+        if (__any(doubt)) {
+            // a group's two best are among those whose q is within the gap of the second
+            const uint32_t second = two ? q1 : q0;
+            double c0 = -INFINITY, c1 = -INFINITY;
+            bool more = doubt && real;
+            unsure |= more && second < gap;
+#pragma unroll 1
+            for (uint32_t i = 0; i < N; i++) {
+                uint32_t key = top[0];
+#pragma unroll
+                for (uint32_t k = 1; k < N; k++) key = i == k ? top[k] : key;
+                more &= (key >> kQShift) + gap > second;
+                if (!__any(more)) break;
+                const uint32_t at = min_u(kk * kPitch + 31u - (key & 31u), kRow - 1u);
+                const double v = more ? choice(score(at), at) : -INFINITY;
+                c1 = fmax(c1, fmin(c0, v));
+                c0 = fmax(c0, v);
+            }
+            if constexpr (L > 1u) unsure |= more;  // there may be one behind the list
+#pragma unroll
+            for (uint32_t st = 1; st < 16u; st <<= 1)
+                if (st < g.of) {
+                    const double o0 = partner_f64(c0, st), o1 = partner_f64(c1, st);
+                    c1 = fmax(fmax(c1, o1), fmin(c0, o0));
+                    c0 = fmax(c0, o0);
+                }
+            const double full = !real ? -INFINITY : two ? c0 + c1 : c0;
+            const bool stays = real && groups_ahead(full, g.of) < r.topk_group;
+            auto least = [](double a, double b) { return fmin(a, b); };
+            const double low = row_reduce_f64(stays ? full : INFINITY, least);
+            const double high = -row_reduce_f64(stays ? INFINITY : -full, least);
+            // scores of at most rz each, and what 64 bits round
+            const double off = r.softmax && !by_logit ? 2.0 * zerr * rz : 0.0;
+            unsure |= doubt && !(low - high > off + 1e-15 * (1.0 + fabs(low)));
+            kept = doubt ? stays : kept;
+        }
+        unsure |= lanes_of(kept) != r.topk_group * g.of;
 #pragma unroll
         for (uint32_t k = 0; k < K; k++) top[k] = kept ? top[k] : 0u;
     }
@@ -484,30 +558,21 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, uint
     const bool crowd = (last >> kQShift) - (then >> kQShift) < gap;
     // The winners are known but for `next`, if it is close to the last of them;
     // lane k_used takes it. Then the order by 64-bit scores, which the weights
-    // take anyway (p + b, whose sum is f32's, by the keys alone)
+    // take anyway
     won = kk == r.k_used ? next : won;
     const bool here = kk < r.k_used, seen = kk <= r.k_used;
-    // (a key of 0, no expert's, stands for one as well: such a row is unsure)
-    const uint32_t id = seen ? min_u((15u - (won >> 5 & 15u)) * per_lane + 31u - (won & 31u), E - 1u) : 0u;
-    const double raw = (double)row_l[place(id)];
-    double w;
-    if (r.softmax) {
-        w = exp(raw - (double)m);
-    } else {
-        const double e = exp(-fabs(raw));
-        w = (raw >= 0.0 ? 1.0 : e) / (1.0 + e);
-    }
-    if (by_logit || !r.softmax) {
-        const double choice = w + (r.bias ? (double)bias_l[place(id)] : 0.0);
-        const bool ahead = choice - row_behind(choice) > 1e-15 * fabs(choice);
-        unsure |= kk + 1u < r.k_used && !ahead;
-        unsure |= close && kk + 1u == r.k_used && (kk == 15u || crowd || !ahead);
-    } else {
-        unsure |= close;
-#pragma unroll
-        for (uint32_t k = 1; k < K; k++)
-            unsure |= k < r.k_used && (top[k - 1u] >> kQShift) - (top[k] >> kQShift) < gap;
-    }
+    // (a key of 0, no expert's, is an unsure row's)
+    const uint32_t from = 15u - (won >> 5 & 15u), nth = 31u - (won & 31u);
+    const uint32_t id = (from >> g.of_log2) * g.size + (from & (g.of - 1u)) * g.per_lane + nth;
+    const uint32_t at = seen ? min_u(from * kPitch + nth, kRow - 1u) : 0u;
+    double w = score(at);
+    const double chosen = choice(w, at), behind = row_behind(chosen);
+    // z's error moves both by as much of their scores
+    double off = r.softmax && !by_logit ? fabs(w - row_behind(w)) * (rz * zerr) : 0.0;
+    off += 1e-15 * (r.bias ? fabs(chosen) + w * rz : fabs(chosen));
+    const bool ahead = chosen - behind > off;
+    unsure |= kk + 1u < r.k_used && !ahead;
+    unsure |= close && kk + 1u == r.k_used && (kk == 15u || crowd || !ahead);
     w = here ? w : 0.0;
     if (r.softmax) {
         const double total = r.renorm ? row_sum(w) : (double)z;
@@ -541,13 +606,17 @@ extern "C" int pulsar_router_select_groups(void *selected, void *weights, const 
         return pk::reject("router select groups");
     const pk::GroupRoute r = {(const float *)logits, (const float *)bias, (int32_t *)selected, (float *)weights,
                               n_expert, k_used, n_group, topk_group, group_top, score, renorm, n_tok, weight_scale};
-    // whole lanes of the 16 a token has: the f32 kernel
-    if (n_expert <= 512u && k_used <= 16u && 16u % n_group == 0u && (n_group == 1u || n_expert % 16u == 0u)) {
-        const uint32_t per_lane = (n_expert + 15u) / 16u;
+    // the f32 kernel: of the 16 lanes of a token, as many to a group as a power of two allows
+    uint32_t of_log2 = 4u;
+    while (of_log2 > 0u && n_group << of_log2 > 16u) of_log2--;
+    const uint32_t of = 1u << of_log2, size = n_expert / n_group;
+    const uint32_t per_lane = (size + of - 1u) / of;
+    if (n_group <= 16u && per_lane <= 32u && n_expert <= 512u && k_used <= 16u) {
+        const pk::GroupLanes lanes = {size, of_log2, of, per_lane, (1u << 20) / size + 1u, (1u << 20) / per_lane + 1u};
         const bool many = n_tok >= 4096u;
 #define PK_RGFK(J, K, W)                                                                                       \
     hipLaunchKernelGGL((pk::route_groups_kernel<J, K, W>), dim3((n_tok + 4u * W - 1u) / (4u * W)), dim3(64u * W), 0, \
-                       pk::stream(), r, per_lane)
+                       pk::stream(), r, lanes)
 #define PK_RGF(J)                               \
     do {                                        \
         constexpr uint32_t kW = J > 16 ? 8 : 16; \

@@ -266,7 +266,7 @@ def moe_group_ids(gptrs, starts, pairs, slot_weights, selected, router_weights, 
             _room(slot_weights, 4 * n_tok * slots, op, "slot_weights", dev),
             _room(selected, 4 * n_tok * k_used, op, "selected", dev),
             _room(router_weights, 4 * n_tok * k_used, op, "router_weights", dev), ctypes.byref(bank), n_expert,
-            ctypes.cast(arr, ctypes.c_void_p), n_shared, n_tok, k_used),
+            arr, n_shared, n_tok, k_used),
         op,
     )
 
@@ -327,12 +327,8 @@ def moe_down_experts(partial, selected, active, midq, bank: "ExpertBank", n_expe
 
 
 def _shared_array(shared):
-    shared = list(shared or [])
-    arr = (_Ptrs6 * max(1, len(shared)))()
-    for i, e in enumerate(shared):
-        e = tuple(e) + (0,) * (6 - len(e))
-        arr[i] = _Ptrs6(*[int(v) or None for v in e])
-    return arr, len(shared)
+    shared = [tuple(map(int, e)) for e in shared or ()]
+    return (_Ptrs6 * max(1, len(shared)))(*shared), len(shared)
 
 
 # ---- fused decode layer (extensions; each equals the separate calls it replaces)

@@ -81,7 +81,8 @@ def check(dev, logits, bias, *how):
 # experts, k, groups, kept groups
 SHAPES = [(1, 1, 1, 1), (8, 2, 4, 2), (32, 4, 1, 1), (64, 6, 8, 3), (91, 13, 1, 1), (104, 13, 8, 2), (128, 8, 1, 1),
           (160, 6, 8, 3), (182, 7, 14, 7), (240, 3, 8, 7), (256, 8, 8, 4), (256, 8, 1, 1), (256, 64, 8, 8),
-          (256, 8, 16, 5), (256, 16, 32, 9), (256, 8, 2, 1), (384, 8, 1, 1), (392, 7, 8, 3), (512, 10, 4, 2),
+          (45, 4, 5, 2), (99, 5, 9, 4), (100, 6, 2, 1), (300, 9, 12, 5), (390, 5, 13, 6), (480, 8, 15, 7),
+          (483, 6, 7, 3), (500, 16, 10, 4), (256, 8, 16, 5), (256, 16, 32, 9), (256, 8, 2, 1), (384, 8, 1, 1), (392, 7, 8, 3), (512, 10, 4, 2),
           (1000, 16, 8, 3), (1024, 64, 64, 11)]
 
 
@@ -134,6 +135,31 @@ def test_next_to_a_border(dev, groups, kept, score):
     for bias in (none, near):
         for group_top in (1, 2):
             check(dev, logits, bias, 8, groups, kept, group_top, score, True, 1.0)
+
+
+@pytest.mark.parametrize("experts,groups,kept", [(256, 8, 4), (120, 6, 2), (256, 16, 15), (60, 2, 1)])
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("score", [SCORE_SIGMOID, SCORE_SOFTMAX])
+def test_groups_next_to_a_border(dev, experts, groups, kept, group_top, score):
+    """Groups whose scores are those of another group, in another order, or a few
+    units in the last place beside them."""
+    rng = np.random.default_rng(experts + group_top)
+    T, size = 120, experts // groups
+    logits = (1.5 * rng.standard_normal((T, groups, size)) - 1.0).astype(np.float32)
+    for t in range(T):
+        a, b = rng.permutation(groups)[:2]
+        logits[t, b] = rng.permutation(logits[t, a])
+        best = np.argsort(logits[t, b])[-group_top:]
+        ulps = [0, 1, -1, 3, -20][t % 5]
+        logits[t, b, best[0]] += ulps * np.spacing(np.abs(logits[t, b, best[0]]))
+        if t % 3 == 1:  # several of the group's best next to one another
+            logits[t, b, rng.permutation(size)[:6]] = logits[t, b, best[-1]] * np.float32(1 + 2.0**-22)
+        if t % 8 == 7:  # all of them
+            logits[t] = logits[t, a]
+    logits = logits.reshape(T, experts)
+    same = np.full(experts, 0.25, np.float32)
+    for bias in (None, same, (0.1 * rng.standard_normal(experts)).astype(np.float32)):
+        check(dev, logits, bias, 6, groups, kept, group_top, score, True, 1.0)
 
 
 @pytest.mark.parametrize("groups,kept,group_top", [(1, 1, 1), (8, 2, 2), (8, 8, 1), (4, 1, 2), (32, 3, 2)])
