@@ -292,10 +292,11 @@ PK_DEV double row_sum(double v) {
     return row_reduce_f64(v, [](double a, double b) { return a + b; });
 }
 // lane i gets lane i + 1 of its row
+PK_DEV uint32_t row_behind(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x101, 0xF, 0xF, true);
+}
 PK_DEV double row_behind(double v) {
-    return halves(v, [](uint32_t h) {
-        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)h, 0x101, 0xF, 0xF, true);
-    });
+    return halves(v, [](uint32_t h) { return row_behind(h); });
 }
 // lane i gets lane (i - N) % 16 of its row
 template <uint32_t N>
@@ -322,6 +323,11 @@ PK_DEV uint32_t groups_ahead(T v, uint32_t of) {  // `of` is uniform
                       : groups_ahead_of<8>(v);
 }
 
+// Blocks start at about one in 4 ns, but of 8 or 16 waves they leave CUs idle
+// where they are not a multiple of the 256: 20000 tokens of 256 experts 9.5 us,
+// 10.9 and 16.6; 16384 8.2, 8.3 and 9.0.
+constexpr uint32_t kRouteWaves = 4;
+
 struct GroupLanes {
     uint32_t size, of_log2, of, per_lane;  // experts and lanes of a group, experts of a lane
     uint32_t by_size, by_lane;  // 2^20 / size and / per_lane, rounded up
@@ -334,11 +340,9 @@ struct GroupLanes {
 };
 
 // J: experts a lane has room for; K: k_used <= K. n_group <= 16.
-// W: waves of a block (blocks start at about one in 4 ns, so a long chunk takes
-// few large ones).
-template <uint32_t J, uint32_t K, uint32_t W>
-__global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, GroupLanes g) {
-    constexpr uint32_t kJ64 = J < 4u ? 1u : J / 4u;
+template <uint32_t J, uint32_t K>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRoute r, GroupLanes g) {
+    constexpr uint32_t W = kRouteWaves, kJ64 = J < 4u ? 1u : J / 4u;
     // A lane's experts in LDS: rows are read from memory as they lie, 16 lanes
     // that read J floats each then find them on distinct banks
     constexpr uint32_t kPitch = J + 4u, kRow = 16u * kPitch;
@@ -357,15 +361,23 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, Grou
                     ld128((const uint8_t *)(r.logits + (uint64_t)token * E + e));
         }
     } else {
-        for (uint32_t i = lane; i < 4u * kRow; i += 64u) mine_l[i] = __builtin_nanf("");  // no expert there
-        __builtin_amdgcn_wave_barrier();  // a wave's LDS writes land in order
-        for (uint32_t e = lane; e < E; e += 64u) {
-            const uint32_t at = g.at(e, kPitch);
+        constexpr uint32_t P = J < 4u ? 1u : J / 4u;  // 64 P >= E
+        float v[P][4];  // all requested before the first is waited for
+#pragma unroll
+        for (uint32_t p = 0; p < P; p++)
 #pragma unroll
             for (uint32_t t = 0; t < 4u; t++) {
                 const uint32_t token = token0 + t < r.n_tok ? token0 + t : r.n_tok - 1u;
-                mine_l[t * kRow + at] = r.logits[(uint64_t)token * E + e];
+                v[p][t] = r.logits[(uint64_t)token * E + min_u(lane + 64u * p, E - 1u)];
             }
+        for (uint32_t i = lane; i < 4u * kRow; i += 64u) mine_l[i] = __builtin_nanf("");  // no expert there
+        __builtin_amdgcn_wave_barrier();  // a wave's LDS writes land in order
+#pragma unroll
+        for (uint32_t p = 0; p < P; p++) {
+            const uint32_t e = lane + 64u * p, at = g.at(e < E ? e : 0u, kPitch);
+#pragma unroll
+            for (uint32_t t = 0; t < 4u; t++)
+                if (e < E) mine_l[t * kRow + at] = v[p][t];
         }
     }
     if (r.bias)
@@ -417,7 +429,7 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, Grou
 #pragma unroll
             for (uint32_t j = 0; j < J; j++) c[j] = x[j] * rz;
             err = 34.0f * rz;
-            window = r.bias ? 1.0f : rz;
+            window = r.bias ? 2.0f : rz;
         }
     } else {
 #pragma unroll
@@ -566,13 +578,24 @@ __global__ __launch_bounds__(64 * W) void route_groups_kernel(GroupRoute r, Grou
     const uint32_t id = (from >> g.of_log2) * g.size + (from & (g.of - 1u)) * g.per_lane + nth;
     const uint32_t at = seen ? min_u(from * kPitch + nth, kRow - 1u) : 0u;
     double w = score(at);
-    const double chosen = choice(w, at), behind = row_behind(chosen);
-    // z's error moves both by as much of their scores
-    double off = r.softmax && !by_logit ? fabs(w - row_behind(w)) * (rz * zerr) : 0.0;
-    off += 1e-15 * (r.bias ? fabs(chosen) + w * rz : fabs(chosen));
-    const bool ahead = chosen - behind > off;
+    const double chosen = choice(w, at);
+    // by how much a choice has to be ahead of that of a score v: what z's error
+    // moves them by, as much of both scores, and what 64 bits round
+    auto margin = [&](double v) {
+        const double off = r.softmax && !by_logit ? fabs(w - v) * (rz * zerr) : 0.0;
+        return off + 1e-15 * (r.bias ? fabs(chosen) + w * rz : fabs(chosen));
+    };
+    // equal ones, of equal logits and biases, lie in the order of their keys, their ids'
+    const uint32_t logit = __float_as_uint(row_l[at]), bias = r.bias ? __float_as_uint(bias_l[at]) : 0u;
+    const bool ahead = chosen - row_behind(chosen) > margin(row_behind(w)) ||
+                       (logit == row_behind(logit) && bias == row_behind(bias));
     unsure |= kk + 1u < r.k_used && !ahead;
-    unsure |= close && kk + 1u == r.k_used && (kk == 15u || crowd || !ahead);
+    unsure |= close && (crowd || (kk + 1u == r.k_used && kk < 15u && !ahead));
+    if (r.k_used == 16u && __any(close)) {  // no lane behind the last one: the two once more
+        const uint32_t at2 = min_u((15u - (next >> 5 & 15u)) * kPitch + 31u - (next & 31u), kRow - 1u);
+        const double w2 = score(at2);
+        unsure |= close && kk == 15u && !(chosen - choice(w2, at2) > margin(w2));
+    }
     w = here ? w : 0.0;
     if (r.softmax) {
         const double total = r.renorm ? row_sum(w) : (double)z;
@@ -613,21 +636,16 @@ extern "C" int pulsar_router_select_groups(void *selected, void *weights, const 
     const uint32_t per_lane = (size + of - 1u) / of;
     if (n_group <= 16u && per_lane <= 32u && n_expert <= 512u && k_used <= 16u) {
         const pk::GroupLanes lanes = {size, of_log2, of, per_lane, (1u << 20) / size + 1u, (1u << 20) / per_lane + 1u};
-        const bool many = n_tok >= 4096u;
-#define PK_RGFK(J, K, W)                                                                                       \
-    hipLaunchKernelGGL((pk::route_groups_kernel<J, K, W>), dim3((n_tok + 4u * W - 1u) / (4u * W)), dim3(64u * W), 0, \
+        constexpr uint32_t W = pk::kRouteWaves;
+#define PK_RGFK(J, K)                                                                                        \
+    hipLaunchKernelGGL((pk::route_groups_kernel<J, K>), dim3((n_tok + 4u * W - 1u) / (4u * W)), dim3(64u * W), 0, \
                        pk::stream(), r, lanes)
-#define PK_RGF(J)                               \
-    do {                                        \
-        constexpr uint32_t kW = J > 16 ? 8 : 16; \
-        if (k_used <= 8u && many)               \
-            PK_RGFK(J, 8, kW);                  \
-        else if (k_used <= 8u)                  \
-            PK_RGFK(J, 8, 4);                   \
-        else if (many)                          \
-            PK_RGFK(J, 16, kW);                 \
-        else                                    \
-            PK_RGFK(J, 16, 4);                  \
+#define PK_RGF(J)          \
+    do {                   \
+        if (k_used <= 8u)  \
+            PK_RGFK(J, 8); \
+        else               \
+            PK_RGFK(J, 16); \
     } while (0)
         if (per_lane <= 1u)
             PK_RGF(1);
