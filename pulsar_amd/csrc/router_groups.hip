@@ -503,7 +503,8 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRou
         const bool real = kk < r.n_group * g.of;
         // a group that stands with one, or with what the window cut, has no sum here
         unsure |= real && two && q1 == 0u;
-        bool kept = real && groups_ahead(stand, g.of) < r.topk_group;
+        const uint32_t rank = groups_ahead(stand, g.of);  // by all lanes: they read one another
+        bool kept = real && rank < r.topk_group;
         const uint32_t last = row_reduce(kept ? stand : UINT32_MAX, min_u), next = row_reduce(kept ? 0u : stand, max_u);
         auto lanes_of = [&](bool b) {  // lanes of the row that say b
             return (uint32_t)__builtin_popcount((uint32_t)(__ballot(b) >> (lane & 48u)) & 0xffffu);
@@ -537,7 +538,8 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRou
                     c0 = fmax(c0, o0);
                 }
             const double full = !real ? -INFINITY : two ? c0 + c1 : c0;
-            const bool stays = real && groups_ahead(full, g.of) < r.topk_group;
+            const uint32_t place = groups_ahead(full, g.of);
+            const bool stays = real && place < r.topk_group;
             auto least = [](double a, double b) { return fmin(a, b); };
             const double low = row_reduce_f64(stays ? full : INFINITY, least);
             const double high = -row_reduce_f64(stays ? INFINITY : -full, least);
@@ -601,8 +603,10 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRou
         chosen = choice(w, at);
         // equal ones, of equal logits and biases, lie in the order of their keys, their ids'
         const uint32_t logit = __float_as_uint(row_l[at]), bias = r.bias ? __float_as_uint(bias_l[at]) : 0u;
+        // (what lanes read of one another is read by all, ahead of any choice)
         const double ahead = chosen - row_behind(chosen), off = margin(row_behind(w));
-        const bool wrong = pair && !(ahead > off || (logit == row_behind(logit) && bias == row_behind(bias)));
+        const uint32_t apart = (logit ^ row_behind(logit)) | (bias ^ row_behind(bias));
+        const bool wrong = pair && !(ahead > off || apart == 0u);
         const uint32_t swap = wrong && ahead < -off ? 1u : 0u;
         if (pass == 3u || !__any(swap != 0u)) {
             unsure |= wrong;
@@ -610,7 +614,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRou
         }
         // two that f32 has in the wrong order change places
         const uint32_t after = row_behind(won), before = row_before(won);
-        const bool down = swap != 0u && row_before(swap) == 0u, up = row_before(down ? 1u : 0u) != 0u;
+        const uint32_t down = swap & ~row_before(swap), up = row_before(down);
         won = down ? after : up ? before : won;
     }
     unsure |= close && crowd;

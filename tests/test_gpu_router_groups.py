@@ -158,7 +158,8 @@ def test_groups_next_to_a_border(dev, experts, groups, kept, group_top, score):
             logits[t] = logits[t, a]
     logits = logits.reshape(T, experts)
     same = np.full(experts, 0.25, np.float32)
-    for bias in (None, same, (0.1 * rng.standard_normal(experts)).astype(np.float32)):
+    near = (0.1 * rng.standard_normal(experts)).astype(np.float32)
+    for bias in (None, same, near, near - np.float32(3), same - np.float32(2)):
         check(dev, logits, bias, 6, groups, kept, group_top, score, True, 1.0)
 
 
