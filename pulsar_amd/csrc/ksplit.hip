@@ -194,7 +194,8 @@ static int launch_ksplit_q(float *out, const uint8_t *w, const pulsar_block_q8_K
 // tokens (Q4_K 4096 x 4096: 33 tokens 8.5 against 11.0 us, 100 tokens 18.9 against
 // 15.2). Below `least` tiles of long rows its blocks leave most CUs idle, and
 // kernels that spread rows further are ahead: the lane kernels, a wave per row
-// (Q3_K 83 x 12032, 2 tokens: 14.7 against 4.4 us), and for Q6_K, whose decode is the longest, the 16-row kernel.
+// (Q3_K 83 x 12032, 2 tokens: 14.7 against 4.4 us), and for Q6_K, whose decode is
+// the longest, the 16-row kernel.
 static bool ksplit_wins(uint32_t quant, uint32_t nb, uint32_t out_dim, uint32_t n_tok) {
     if (n_tok == 1u) return false;
     const uint64_t tiles = ksplit_tiles(out_dim, n_tok);

@@ -59,7 +59,7 @@ def _room(buf, nbytes: int, op: str, what: str, device: int) -> int:
     """The device address of `buf`, which the launch uses the first nbytes
     bytes of; a tensor has to be contiguous, that large and on the current
     device (a raw address is the caller's word for all three)."""
-    if buf is None or type(buf) is int:
+    if buf is None or not hasattr(buf, "data_ptr"):
         return _ptr(buf)
     if buf.get_device() != device:
         _misplaced(buf, op, what)
@@ -83,7 +83,7 @@ def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str, device: i
     """The device address of n_rows rows of dim floats, `stride` floats apart.
     A tensor may be a view of columns of a wider array: it has to be f32 [..,
     dim] with that stride, or contiguous and large enough."""
-    if buf is None or type(buf) is int:
+    if buf is None or not hasattr(buf, "data_ptr"):
         return _ptr(buf)
     if buf.get_device() != device:
         _misplaced(buf, op, what)
