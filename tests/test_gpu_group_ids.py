@@ -184,6 +184,25 @@ def test_captured(dev, T):
         assert np.array_equal(down(s), starts) and np.array_equal(down(p), pairs)
 
 
+@pytest.mark.parametrize("T", [700, 20000])
+def test_own_stream(dev, T):
+    k, E = 4, 40
+    ids = np.random.default_rng(10).integers(0, E, (T, k)).astype(np.int32)
+    sel = torch.from_numpy(ids).to(dev)
+    g = torch.zeros((E, 6), dtype=torch.int64, device=dev)
+    s, p = torch.zeros(E + 1, dtype=torch.int32, device=dev), torch.zeros(T * k, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    K.set_stream(stream)
+    try:
+        K.moe_group_ids(g, s, p, None, sel, None, bank_of(False), E, None, T, k)
+    finally:
+        K.set_stream(None)
+    stream.synchronize()
+    starts, pairs = want_long(ids, E, 0)
+    assert np.array_equal(down(s), starts) and np.array_equal(down(p), pairs)
+
+
 def test_wrapper_refuses_short_tensors(dev):
     z = torch.zeros(4096, dtype=torch.int32, device=dev)
     good = dict(gptrs=z, starts=z, pairs=z, slot_weights=z, selected=z, router_weights=z)

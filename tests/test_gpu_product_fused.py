@@ -253,6 +253,21 @@ def test_own_stream(dev):
     assert np.array_equal(down(out), want)
 
 
+@pytest.mark.parametrize("T", [4, 5, 33])
+def test_rows_past_32_bit_offsets(dev, T):
+    """Rows of out and residual so far apart that the last one starts behind 4 GiB."""
+    c = Case(fm.QUANT_Q6_K, 100, 512, T)
+    stride = 2**30 // (T - 1) + 7  # floats
+    wide = torch.zeros((T - 1) * stride + 100, device=dev)
+    out = wide.as_strided((T, 100), (stride, 1))
+    out.copy_(up_f32(c.res))
+    torch.cuda.synchronize()
+    c.run(out, up_f32(c.bias), out, EPI_NONE, out_stride=stride, res_stride=stride)
+    runtime.sync()
+    assert_epilogue(down(out.contiguous()), c.dots, c.bias, EPI_NONE, c.res, T)
+    assert not wide[100:stride].any()
+
+
 def test_wrapper_refuses_short_tensors(dev):
     c = Case(fm.QUANT_Q4_K, 64, 256, 4)
     z = torch.zeros((4, 64), device=dev)

@@ -236,6 +236,39 @@ def test_captured(dev):
         assert (down(ids) == want).all() and (down(w) == wts).all()
 
 
+def test_own_stream(dev):
+    rng = np.random.default_rng(6)
+    T, E, k = 70, 256, 8
+    logits = rng.standard_normal((T, E)).astype(np.float32)
+    want, wts = run(dev, logits, None, k, 8, 4, 2, SCORE_SIGMOID, True, 1.0)
+    x, ids, w = up_f32(logits), torch.zeros((T, k), dtype=torch.int32, device=dev), torch.zeros((T, k), device=dev)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    K.set_stream(stream)
+    try:
+        K.router_select_groups(ids, w, x, None, E, k, 8, 4, 2, SCORE_SIGMOID, True, 1.0, T)
+    finally:
+        K.set_stream(None)
+    stream.synchronize()
+    assert (down(ids) == want).all() and (down(w) == wts).all()
+
+
+@pytest.mark.parametrize("groups", [8, 32])
+def test_logits_past_32_bit_offsets(dev, groups):
+    T, E, k = 2**21 + 5, 512, 4
+    x = torch.empty((T, E), device=dev).normal_(generator=torch.Generator(device=dev).manual_seed(7))
+    ids, w = torch.full((T, k), -7, dtype=torch.int32, device=dev), torch.full((T, k), math.nan, device=dev)
+    torch.cuda.synchronize()
+    how = (k, groups, 3, 2, SCORE_SOFTMAX, True, 1.0)
+    K.router_select_groups(ids, w, x, None, E, *how, T)
+    runtime.sync()
+    at = [0, 2**20 - 1, 2**21 - 1, 2**21, T - 1]
+    want, wts, tol = want_route(down(x[at]), None, *how)
+    assert (down(ids[at]) == want).all()
+    assert (np.abs(down(w[at]) - wts) <= tol).all()
+    assert int(ids.min()) >= 0
+
+
 def test_wrapper_refuses_short_tensors(dev):
     z = torch.zeros(4 * 32, device=dev)
     ids = torch.zeros(4 * 4, dtype=torch.int32, device=dev)
