@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void route_groups_f64_kernel(GroupRoute r) {
 // one behind them if it is close, are then put to the test by their 64-bit
 // scores. A row that fails one (ties, an order that f32 swapped), that has
 // infinite scores or runs out of candidates or of the window, is done again by
-// route_token_f64: rows of ties always, a trained router's hardly ever.
+// route_token_f64: a row of many ties, a trained router's hardly ever.
 
 constexpr uint32_t kQShift = 9;  // below q: 15 - kk in 4 bits, 31 - j in 5
 constexpr float kSteps = 8384000.0f;  // q < 2^23, with room for 4600 steps of rounding
