@@ -1,0 +1,96 @@
+"""What the wrappers of the routing with expert groups, the grouping by ids and the
+product with an epilogue refuse of a tensor or a number, before the library is
+called (no GPU: stand-ins for device tensors, whose memory is never read)."""
+import pytest
+import torch
+
+from pulsar_amd import _lib
+from pulsar_amd import kernels as K
+from pulsar_amd.formats import QUANT_Q4_K
+
+
+@pytest.fixture(scope="module", autouse=True)
+def lib():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("the library is not built")
+    return _lib.load()
+
+
+class Placed:
+    """A tensor without memory, on the current device at an address of its own."""
+
+    is_cuda = True
+    taken = 0
+
+    def __init__(self, shape, dtype):
+        self.t = torch.empty(shape, dtype=dtype, device="meta")
+        Placed.taken += 1
+        self.address = Placed.taken << 32
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return K._device()
+
+    def data_ptr(self):
+        return self.address
+
+
+I32, F32 = torch.int32, torch.float32
+T, E, N = 3, 32, 4
+
+
+def route(**change):
+    a = dict(selected=Placed((T, N), I32), weights=Placed((T, N), F32), logits=Placed((T, E), F32),
+             bias=Placed((E,), F32), n_expert=E, k_used=N, n_group=8, topk_group=2, group_top=2, score=0, renorm=True,
+             weight_scale=1.0, n_tok=T)
+    K.router_select_groups(**{**a, **change})
+
+
+def group(**change):
+    a = dict(gptrs=Placed((E, 6), torch.int64), starts=Placed((E + 1,), I32), pairs=Placed((T * N,), I32),
+             slot_weights=Placed((T, N), F32), selected=Placed((T, N), I32), router_weights=Placed((T, N), F32),
+             bank=K.ExpertBank(1 << 20, 2 << 20, 3 << 20, None, None, None, 64, 64, 64, 0, 0, 0), n_expert=E,
+             shared=[], n_tok=T, k_used=N)
+    K.moe_group_ids(**{**a, **change})
+
+
+ROWS, COLS, RB = 64, 512, 288
+
+
+def product(**change):
+    a = dict(out=Placed((T, ROWS), F32), w=Placed((ROWS, RB), torch.uint8), xq=Placed((T, 584), torch.uint8),
+             bias=Placed((ROWS,), F32), residual=Placed((T, ROWS), F32), in_dim=COLS, out_dim=ROWS, n_tok=T,
+             row_bytes=RB, quant=QUANT_Q4_K)
+    K.matmul_kq_fused(**{**a, **change})
+
+
+@pytest.mark.parametrize("call", [route, group, product])
+def test_sound_arguments_reach_the_library(call):
+    """What the refusals below are told apart from: without a GPU the launch
+    itself fails."""
+    if torch.cuda.is_available():
+        pytest.skip("these addresses are nobody's")
+    with pytest.raises(K.KernelError):
+        call()
+
+
+WIDE = [(route, "selected", (T, N), torch.int64), (route, "selected", (T, N), F32),
+        (route, "weights", (T, N), torch.float64), (route, "weights", (T, 2 * N), torch.float16),
+        (route, "logits", (T, E), torch.float64), (route, "logits", (T, 2 * E), torch.bfloat16),
+        (route, "bias", (E,), torch.float64), (route, "bias", (E,), I32),
+        (group, "starts", (E + 1,), torch.int64), (group, "pairs", (T * N,), torch.int64),
+        (group, "selected", (T, N), torch.int64), (group, "selected", (T, 2 * N), torch.int16),
+        (group, "router_weights", (T, N), torch.float64), (group, "router_weights", (T, 2 * N), torch.bfloat16),
+        (group, "slot_weights", (T, N), torch.float64), (group, "slot_weights", (T, N), I32),
+        (product, "bias", (ROWS,), torch.float64), (product, "bias", (2 * ROWS,), torch.float16),
+        (product, "out", (T, ROWS), I32), (product, "residual", (T, ROWS), I32)]
+
+
+@pytest.mark.parametrize("call,name,shape,dtype", WIDE)
+def test_refuses_other_element_types(call, name, shape, dtype):
+    """Large enough, but of a type whose bytes are not the operator's numbers:
+    torch.topk's int64 ids are the case that a router meets."""
+    with pytest.raises(ValueError, match=f"{name} has to be"):
+        call(**{name: Placed(shape, dtype)})
