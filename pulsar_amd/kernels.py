@@ -16,7 +16,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from .formats import BLOCK_LAYOUT, EXPERT_PTRS_BYTES
+from .formats import BLOCK_LAYOUT, EXPERT_PTRS_BYTES, QUANT_A4_OK
 
 
 class KernelError(RuntimeError):
@@ -119,7 +119,7 @@ def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok
     bias) + residual[t] (formats.EPI_* codes; bias and residual may be None).
     Strides in floats, 0 for packed rows; residual may be out itself."""
     op, dev = "matmul_kq_fused", _device()
-    block, block_bytes = BLOCK_LAYOUT.get(quant, (1, 0))
+    block, block_bytes = BLOCK_LAYOUT.get(quant & ~QUANT_A4_OK, (1, 0))
     w_bytes = (out_dim - 1) * row_bytes + in_dim // block * block_bytes
     xq_bytes, so, sr = n_tok * -(-in_dim // 256) * 292, out_stride or out_dim, res_stride or out_dim
     other = []

@@ -6,7 +6,7 @@ import torch
 
 from pulsar_amd import _lib
 from pulsar_amd import kernels as K
-from pulsar_amd.formats import QUANT_Q4_K
+from pulsar_amd.formats import DENSE_QUANTS, QUANT_A4_OK, QUANT_Q4_K, row_bytes
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -94,3 +94,15 @@ def test_refuses_other_element_types(call, name, shape, dtype):
     torch.topk's int64 ids are the case that a router meets."""
     with pytest.raises(ValueError, match=f"{name} has to be"):
         call(**{name: Placed(shape, dtype)})
+
+
+@pytest.mark.parametrize("flag", [0, QUANT_A4_OK])
+@pytest.mark.parametrize("quant", DENSE_QUANTS)
+def test_refuses_weights_short_of_their_last_row(quant, flag):
+    """With and without the flag beside the format's code, which the library
+    takes off before it reads the rows."""
+    rb = row_bytes(quant, COLS)
+    xq = Placed((T, 584), torch.uint8)
+    for n in ((ROWS - 1) * rb, ROWS * rb - 1):
+        with pytest.raises(ValueError, match="w has to be contiguous"):
+            product(w=Placed((n,), torch.uint8), xq=xq, row_bytes=rb, quant=quant | flag)
