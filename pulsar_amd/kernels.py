@@ -77,6 +77,11 @@ def _room(buf, nbytes: int, op: str, what: str, device: int, types=None, other=N
     return buf.data_ptr()
 
 
+def _out_of_range(op: str) -> None:
+    """A number that ctypes would cut to its low bits, -1 to the largest one."""
+    raise ValueError(f"{op}: a size or code is out of range")
+
+
 def _refuse(op: str, other) -> None:
     what, want, got = other[0]
     raise ValueError(f"{op}: {what} has to be {want} (got {got})")
@@ -119,6 +124,8 @@ def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok
     bias) + residual[t] (formats.EPI_* codes; bias and residual may be None).
     Strides in floats, 0 for packed rows; residual may be out itself."""
     op, dev = "matmul_kq_fused", _device()
+    if (in_dim | out_dim | n_tok | quant | act) >> 32 or (row_bytes | out_stride | res_stride) >> 64:
+        _out_of_range(op)
     block, block_bytes = BLOCK_LAYOUT.get(quant & ~QUANT_A4_OK, (1, 0))
     w_bytes = (out_dim - 1) * row_bytes + in_dim // block * block_bytes
     xq_bytes, so, sr = n_tok * -(-in_dim // 256) * 292, out_stride or out_dim, res_stride or out_dim
@@ -207,6 +214,8 @@ def router_select_groups(selected, weights, logits, bias, n_expert: int, k_used:
     (a group's score: its group_top largest score + bias; formats.SCORE_*),
     the weights the winners' scores, renormalised if renorm, times weight_scale."""
     op, dev, other = "router_select_groups", _device(), []
+    if (n_expert | k_used | n_group | topk_group | group_top | score | n_tok) >> 32:
+        _out_of_range(op)
     arrays = (_room(selected, 4 * n_tok * k_used, op, "selected", dev, _I32, other),
               _room(weights, 4 * n_tok * k_used, op, "weights", dev, _F32, other),
               _room(logits, 4 * n_tok * n_expert, op, "logits", dev, _F32, other),
@@ -271,6 +280,8 @@ def moe_group_ids(gptrs, starts, pairs, slot_weights, selected, router_weights, 
     with n_group = n_expert + len(shared). slot_weights (None: left out) gets
     router_weights and the shared slots' ones."""
     op, dev, other = "moe_group_ids", _device(), []
+    if (n_expert | n_tok | k_used) >> 32:
+        _out_of_range(op)
     arr, n_shared = _shared_array(shared)
     groups, slots = n_expert + n_shared, k_used + n_shared
     arrays = (_room(gptrs, EXPERT_PTRS_BYTES * groups, op, "gptrs", dev),

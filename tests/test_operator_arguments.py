@@ -106,3 +106,22 @@ def test_refuses_weights_short_of_their_last_row(quant, flag):
     for n in ((ROWS - 1) * rb, ROWS * rb - 1):
         with pytest.raises(ValueError, match="w has to be contiguous"):
             product(w=Placed((n,), torch.uint8), xq=xq, row_bytes=rb, quant=quant | flag)
+
+
+@pytest.mark.parametrize("call,names", [
+    (route, ("n_expert", "k_used", "n_group", "topk_group", "group_top", "score", "n_tok")),
+    (group, ("n_expert", "n_tok", "k_used")),
+    (product, ("in_dim", "out_dim", "n_tok", "row_bytes", "quant", "act", "out_stride", "res_stride"))])
+def test_refuses_numbers_that_the_library_would_read_as_others(call, names):
+    """Below 0 every array is large enough, and the library reads the low bits:
+    -1 token as 4294967295, 2^32 + 1 as one."""
+    with_u64 = {"row_bytes", "out_stride", "res_stride"}
+    for name in names:
+        bits = 64 if name in with_u64 else 32
+        for value in (-1, -256, 2**bits, 2**bits + 1):
+            with pytest.raises(ValueError, match="out of range"):
+                call(**{name: value})
+            # of raw addresses too, whose sizes nothing else checks
+            with pytest.raises(ValueError, match="out of range"):
+                call(**{name: value, **{a: 1 << 40 for a in ("weights", "selected", "logits", "bias") if call is route},
+                        **{a: 1 << 40 for a in ("out", "w", "xq") if call is product}})
