@@ -313,8 +313,10 @@ int pulsar_moe_group_csr(void *gptrs, void *starts, void *pairs, const void *ptr
  * where NULL: router_weights [n_tok][k_used], then 1 for the shared slots.
  * n_expert <= 1024, k_used + n_shared <= 16, n_shared <= 4, n_tok <= 2^28,
  * n_tok * (k_used + n_shared) < 2^31; bank and shared are host pointers read at
- * launch. gptrs and starts are working memory too while the call runs: two
- * calls that may run at once take buffers of their own. */
+ * launch. An output over an input or another output is refused, but for
+ * slot_weights that are router_weights themselves where n_shared is 0. gptrs and
+ * starts are working memory too while the call runs: two calls that may run at
+ * once take buffers of their own. */
 int pulsar_moe_group_ids(void *gptrs, void *starts, void *pairs, void *slot_weights,
                          const void *selected, const void *router_weights,
                          const pulsar_expert_bank *bank, uint32_t n_expert,

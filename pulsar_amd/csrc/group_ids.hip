@@ -293,6 +293,24 @@ extern "C" int pulsar_moe_group_ids(void *gptrs, void *starts, void *pairs, void
         n_expert > 64u * pk::kMaxPerLane || n_shared > pk::kMaxShared || (n_shared && !shared) || n_tok == 0 ||
         n_tok > 1u << 28 || k_used == 0 || k_used > 16u || k_used + n_shared > 16u || n_slot > 0x7fffffffull)
         return pk::reject("moe group ids");
+    // Blocks still read the ids and weights as others write, and hand their counts
+    // over in gptrs and starts. Weights copied onto themselves are each read and
+    // written by one thread
+    struct {
+        const void *at;
+        pk::u128 bytes;
+    } const out[4] = {{gptrs, sizeof(pulsar_expert_ptrs) * (pk::u128)(n_expert + n_shared)},
+                      {starts, 4 * (pk::u128)(n_expert + n_shared + 1u)},
+                      {pairs, 4 * (pk::u128)n_slot},
+                      {slot_weights, slot_weights ? 4 * (pk::u128)n_slot : 0}};
+    const pk::u128 in_bytes = 4 * (pk::u128)n_tok * k_used;
+    for (uint32_t i = 0; i < (slot_weights ? 4u : 3u); i++) {
+        bool over = pk::overlap(out[i].at, out[i].bytes, selected, in_bytes);
+        if (slot_weights && !(i == 3u && slot_weights == router_weights && n_shared == 0u))
+            over |= pk::overlap(out[i].at, out[i].bytes, router_weights, in_bytes);
+        for (uint32_t j = 0; j < i; j++) over |= pk::overlap(out[i].at, out[i].bytes, out[j].at, out[j].bytes);
+        if (over) return pk::reject("moe group ids (overlap)");
+    }
     pk::GroupIds a = {(pulsar_expert_ptrs *)gptrs, (uint32_t *)starts, (uint32_t *)pairs, (float *)slot_weights,
                       (const int32_t *)selected, (const float *)router_weights, *bank, {}, n_expert, n_shared, n_tok,
                       k_used};

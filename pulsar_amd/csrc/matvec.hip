@@ -265,12 +265,6 @@ static int dense_product(const char *what, void *out, const void *w, const void 
 #undef PK_MVQ
 }
 
-// Bytes [a, a + an) and [b, b + bn) share one
-typedef unsigned __int128 u128;
-static bool overlap(const void *a, u128 an, const void *b, u128 bn) {
-    return (u128)(uintptr_t)a < (uintptr_t)b + bn && (u128)(uintptr_t)b < (uintptr_t)a + an;
-}
-
 // Whether the rows of out may be written while those of residual are read:
 // the same rows (an element is read before it is written), apart, or columns
 // of one wider array that share no float.

@@ -35,6 +35,12 @@ static inline int reject(const char *what) {
     return 0;
 }
 
+// Bytes [a, a + an) and [b, b + bn) share one
+typedef unsigned __int128 u128;
+static inline bool overlap(const void *a, u128 an, const void *b, u128 bn) {
+    return (u128)(uintptr_t)a < (uintptr_t)b + bn && (u128)(uintptr_t)b < (uintptr_t)a + an;
+}
+
 // A pointer read from memory (expert tables) is generic to the compiler;
 // this marks it as global memory so loads through it are global loads.
 PK_DEV const uint8_t *as_global(const void *p) {

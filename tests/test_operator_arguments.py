@@ -125,3 +125,45 @@ def test_refuses_numbers_that_the_library_would_read_as_others(call, names):
             with pytest.raises(ValueError, match="out of range"):
                 call(**{name: value, **{a: 1 << 40 for a in ("weights", "selected", "logits", "bias") if call is route},
                         **{a: 1 << 40 for a in ("out", "w", "xq") if call is product}})
+
+
+# what an entry point says of overlapping arrays on stderr, before any launch
+def refused(capfd, call):
+    capfd.readouterr()
+    with pytest.raises(K.KernelError):
+        call()
+    return "(overlap): invalid arguments" in capfd.readouterr().err
+
+
+def apart(sizes):
+    """Addresses in a row with nothing between the arrays."""
+    at, out = 1 << 40, {}
+    for name, n in sizes.items():
+        out[name], at = at, at + n
+    return out
+
+
+def test_grouping_refuses_arrays_over_one_another(capfd):
+    if torch.cuda.is_available():
+        pytest.skip("these addresses are nobody's")
+    shared = [(16, 32, 48)]
+    slots = N + 1
+    size = dict(gptrs=48 * (E + 1), starts=4 * (E + 2), pairs=4 * T * slots, slot_weights=4 * T * slots,
+                selected=4 * T * N, router_weights=4 * T * N)
+    at = apart(size)
+    assert not refused(capfd, lambda: group(shared=shared, **at))
+    outs = ("gptrs", "starts", "pairs", "slot_weights")
+    for a in outs:
+        for b in size:
+            if b == a:
+                continue
+            for address in (at[b], at[b] + size[b] - 4, at[b] - size[a] + 4):
+                call = {**at, a: address}
+                assert refused(capfd, lambda: group(shared=shared, **call)), (a, b, address - at[b])
+    # a copy onto itself is none where every slot is the router's
+    own = {**at, "slot_weights": at["router_weights"]}
+    assert not refused(capfd, lambda: group(shared=[], **own))
+    assert refused(capfd, lambda: group(shared=shared, **own))
+    # weights that are not asked for are not read
+    own = {**at, "slot_weights": 0, "router_weights": at["pairs"]}
+    assert not refused(capfd, lambda: group(shared=shared, **own))
