@@ -236,7 +236,8 @@ int pulsar_router_select(void *selected, void *weights, const void *logits,
  *     all 0 where every winner's s is 0 in 64 bits); times weight_scale
  * Ids are decided as c stands in 64 bits, whatever f32 would round it to.
  * n_expert <= 1024, a multiple of n_group <= 64; k_used <= 64 and <= the
- * experts of topk_group groups; n_tok <= 2^25. */
+ * experts of topk_group groups; n_tok <= 2^25. selected and weights over one
+ * another, the logits or the bias are refused. */
 int pulsar_router_select_groups(void *selected, void *weights, const void *logits,
                                 const void *bias, uint32_t n_expert, uint32_t k_used,
                                 uint32_t n_group, uint32_t topk_group, uint32_t group_top,

@@ -654,6 +654,13 @@ extern "C" int pulsar_router_select_groups(void *selected, void *weights, const 
         topk_group > n_group || group_top == 0 || group_top > 2u || k_used == 0 || k_used > 64u ||
         k_used > n_expert / n_group * topk_group || score > 1u)
         return pk::reject("router select groups");
+    // other tokens' logits and the bias are still read as a token's results are written
+    const pk::u128 out_bytes = 4 * (pk::u128)n_tok * k_used, in_bytes = 4 * (pk::u128)n_tok * n_expert;
+    bool over = pk::overlap(selected, out_bytes, weights, out_bytes);
+    for (const void *out : {selected, weights})
+        over |= pk::overlap(out, out_bytes, logits, in_bytes) ||
+                (bias && pk::overlap(out, out_bytes, bias, 4 * (pk::u128)n_expert));
+    if (over) return pk::reject("router select groups (overlap)");
     const pk::GroupRoute r = {(const float *)logits, (const float *)bias, (int32_t *)selected, (float *)weights,
                               n_expert, k_used, n_group, topk_group, group_top, score, renorm, n_tok, weight_scale};
     // the f32 kernel: of the 16 lanes of a token, as many to a group as a power of two allows

@@ -167,3 +167,22 @@ def test_grouping_refuses_arrays_over_one_another(capfd):
     # weights that are not asked for are not read
     own = {**at, "slot_weights": 0, "router_weights": at["pairs"]}
     assert not refused(capfd, lambda: group(shared=shared, **own))
+
+
+def test_routing_refuses_outputs_over_its_arrays(capfd):
+    if torch.cuda.is_available():
+        pytest.skip("these addresses are nobody's")
+    size = dict(selected=4 * T * N, weights=4 * T * N, logits=4 * T * E, bias=4 * E)
+    at = apart(size)
+    assert not refused(capfd, lambda: route(**at))
+    for a in ("selected", "weights"):
+        for b in size:
+            if b == a:
+                continue
+            for address in (at[b], at[b] + size[b] - 4, at[b] - size[a] + 4):
+                call = {**at, a: address}
+                assert refused(capfd, lambda: route(**call)), (a, b, address - at[b])
+    at["bias"] = 0
+    assert not refused(capfd, lambda: route(**at))
+    at["bias"] = at["logits"] + 4 * E  # a row of the logits, which is only read
+    assert not refused(capfd, lambda: route(**at))
