@@ -316,6 +316,21 @@ template <uint32_t N>
 PK_DEV double row_turn(double v) {
     return halves(v, [](uint32_t h) { return row_turn<N>(h); });
 }
+
+// e^(l - m) for finite l <= m, within 2^-33 of itself: y = (l - m) log2(e) = n + f,
+// 2^f = 1 + f g(f), g the polynomial through (2^f - 1) / f at the 7 Chebyshev
+// points of |f| <= 1/2. 0, to any sum with e^0 in it, where l is NaN or far below m
+PK_DEV double exp_below(float l, double m) {
+    constexpr double g[7] = {0.69314718055994495,   0.2402265092228883,    0.055504108839093055,  0.0096180566785164946,
+                             0.0013333502386613757, 0.00015461444699823332, 1.5297323668109702e-05};
+    const double y = fmax(((double)l - m) * 1.4426950408889634, -1020.0), n = __builtin_rint(y), f = y - n;
+    double p = g[6];
+#pragma unroll
+    for (int i = 5; i >= 0; i--) p = __builtin_fma(p, f, g[i]);
+    const uint64_t power = (uint64_t)((int32_t)n + 1023) << 52;  // 2^n, n in [-1020, 0]
+    return __builtin_fma(p, f, 1.0) * __builtin_bit_cast(double, power);
+}
+
 // how many of the row's other groups, of G lanes each, have a larger v
 template <uint32_t G, uint32_t N = G, typename T>
 PK_DEV uint32_t groups_ahead_of(T v) {
@@ -399,6 +414,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRou
     // from the exact one, in steps of 2^-24
     float c[J], err, window;
     float m = 0.0f, z = 1.0f;
+    double total = 1.0;
     bool unsure = false;
     constexpr float kLog2e = 1.4426950408889634f;
     const bool by_logit = r.softmax && !r.bias && (r.n_group == 1u || r.group_top == 1u);
@@ -414,7 +430,20 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRou
         m = row_max_f(m);
         unsure = !(fabsf(m) < INFINITY);
         float x[J];
-        if (!by_logit || !r.renorm) {
+        if (!r.renorm) {
+            // total divides the weights, and f32's sum of exps is off by more than the
+            // half step that rounds them. 16384 tokens of 256 experts: 11.0 us, in 8
+            // groups 12.4, by f32's sum 9.3 and 10.8
+            total = 0.0;
+#pragma unroll
+            for (uint32_t j = 0; j < J; j++) {
+                const double term = exp_below(c[j], (double)m);
+                total += term;
+                x[j] = __builtin_fmaf(c[j], 0.0f, (float)term);  // NaN stays
+            }
+            total = row_sum(total);
+            z = (float)total;
+        } else if (!by_logit) {
             float sum[J];
 #pragma unroll
             for (uint32_t j = 0; j < J; j++) {
@@ -625,7 +654,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_groups_kernel(GroupRou
     }
     w = here ? w : 0.0;
     if (r.softmax) {
-        const double total = r.renorm ? row_sum(w) : (double)z;
+        if (r.renorm) total = row_sum(w);
         w = total > 0.0 ? w / total : 0.0;  // as far below the row's best as 64 bits reach: 0
     } else if (r.renorm) {
         w /= fmax(row_sum(w), 6.103515625e-5);
