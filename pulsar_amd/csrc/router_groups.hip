@@ -181,7 +181,7 @@ PK_DEV void route_token_f64(const GroupRoute &r, uint32_t token, double *c_l) {
     }
     if (lane < r.k_used) {
         r.selected[(uint64_t)token * r.k_used + lane] = id;
-        r.weights[(uint64_t)token * r.k_used + lane] = (float)(ws * (double)r.scale);
+        r.weights[(uint64_t)token * r.k_used + lane] = id < 0 ? 0.0f : (float)(ws * (double)r.scale);
     }
 }
 

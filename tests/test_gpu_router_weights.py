@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from pulsar_amd.formats import SCORE_SOFTMAX
+from pulsar_amd.formats import SCORE_SIGMOID, SCORE_SOFTMAX
 from tests.test_gpu_router_groups import run, want_route
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +31,19 @@ def test_softmax_without_renormalisation(dev, experts, k, groups, kept, spread):
         err = np.abs(w - wts)
         bound = wts * (2.0**-24 + 2.0**-32) + 2.0**-149
         assert (err <= bound).all(), float((err / np.maximum(wts, 1e-300)).max() * 2**24)
+
+
+@pytest.mark.parametrize("experts,groups,kept", [(64, 8, 2), (1000, 1, 1)])
+@pytest.mark.parametrize("score", [SCORE_SIGMOID, SCORE_SOFTMAX])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("scale", [np.inf, -np.inf, np.nan])
+def test_empty_slots_under_any_scale(dev, experts, groups, kept, score, renorm, scale):
+    """A slot that no expert is left for is -1 with weight 0, times whatever."""
+    logits = np.full((5, experts), -np.inf, np.float32)
+    logits[1, 3], logits[2, [1, 2]], logits[3] = 1.0, 0.5, np.nan
+    for bias in (None, np.zeros(experts, np.float32)):
+        ids, w = run(dev, logits, bias, 4, groups, kept, 1, score, renorm, scale)
+        assert (ids[[0, 3, 4]] == -1).all() and ids[1].tolist() == [3, -1, -1, -1] and ids[2].tolist() == [1, 2, -1, -1]
+        assert (w[ids == -1] == 0.0).all(), w
+        won = w[ids >= 0]
+        assert np.isnan(won).all() if np.isnan(scale) else (won == scale).all()
