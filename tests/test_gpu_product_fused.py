@@ -88,8 +88,8 @@ class Case:
 
 
 # rows, values, tokens: the lane kernels (1 to 4 tokens, several rows to a wave,
-# rows of more than 8 units a lane), the 16-row kernel, each wide tile, the K split
-# with every width of its token tile and more and fewer super-blocks than waves
+# rows of more than 8 units a lane), the 16-row kernel, the wide tile, the K split
+# (each form of these two for each format: tests/test_gpu_product_forms.py)
 SHAPES = [(1, 256, 1), (33, 512, 1), (500, 4096, 1), (5000, 256, 1), (65, 33024, 1), (40, 33024, 3), (130, 8448, 2),
           (70, 16640, 4), (301, 768, 3), (16500, 512, 2), (100, 512, 5), (8200, 256, 16), (16500, 768, 12),
           (513, 1024, 31), (70, 4352, 14), (4129, 512, 33), (8300, 512, 49), (1000, 768, 70), (1100, 2816, 100),
