@@ -308,7 +308,12 @@ int pulsar_moe_group_csr(void *gptrs, void *starts, void *pairs, const void *ptr
  * token. Writes gptrs [n_expert + n_shared], starts [n_expert + n_shared + 1]
  * and pairs [starts[n_expert + n_shared]] (room for n_tok * (k_used + n_shared);
  * what lies behind the last pair is left as it is), for the grouped stages with
- * n_group = n_expert + n_shared and n_used = k_used + n_shared. selected int32
+ * n_group = n_expert + n_shared and n_used = k_used + n_shared. Those have a fast
+ * path for long groups up to n_group = 1024: behind 1024 experts, call them once on
+ * the first 1024 groups and once on the shared slots' (gptrs and starts + 1024,
+ * n_group = n_shared, the same pairs), which writes the same rows. 8192 tokens of
+ * 8 + 1 slots, 2048 x 512 values: gate / up 0.9 ms in two calls, 12.4 in one for
+ * Q4_K, 81 for IQ4_XS. selected int32
  * [n_tok][k_used]; ids outside [0, n_expert) get no pair, so the caller zeroes
  * partial as for any CSR. slot_weights f32 [n_tok][k_used + n_shared], left out
  * where NULL: router_weights [n_tok][k_used], then 1 for the shared slots.

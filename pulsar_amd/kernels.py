@@ -277,8 +277,10 @@ def moe_group_ids(gptrs, starts, pairs, slot_weights, selected, router_weights, 
                   shared, n_tok: int, k_used: int) -> None:
     """The CSR by expert of a chunk of any length from the router's ids: group e
     is bank expert e, then one group per shared slot; the grouped stages take it
-    with n_group = n_expert + len(shared). slot_weights (None: left out) gets
-    router_weights and the shared slots' ones."""
+    with n_group = n_expert + len(shared), in two calls where that is above 1024
+    (gptrs and starts of the groups behind 1024 in the second): one leaves their
+    fast path. slot_weights (None: left out) gets router_weights and the shared
+    slots' ones."""
     op, dev, other = "moe_group_ids", _device(), []
     if (n_expert | n_tok | k_used) >> 32:
         _out_of_range(op)

@@ -89,3 +89,36 @@ def test_layer(dev, T, E, k, G, kept, n_shared, empty, score):
             assert_rows_close(hpart[i, s], v.reshape(-1), bound.reshape(-1), f"down {t} {s} {e}")
     total, size = hpart.astype(np.float64).sum(1), np.abs(hpart.astype(np.float64)).sum(1)
     assert (np.abs(sums[at] - total) <= slots * 2.0**-24 * size).all()  # a rounding an addition
+
+
+@pytest.mark.parametrize("quant", [GQ, DQ])
+def test_stages_in_slices_of_the_groups(dev, quant):
+    """1024 experts and two shared slots, the grouped stages called on 1024 groups
+    and on the two behind them, whose starts go on where the others' end: the rows
+    of one call on all."""
+    T, E, k, n_shared, hidden, ffn = 3300, 1024, 4, 2, 512, 256
+    rng = np.random.default_rng(5)
+    slots, groups, n = k + n_shared, E + n_shared, T * (k + n_shared)
+    rbs, kinds = (row_bytes(quant, hidden), row_bytes(quant, ffn)), 23
+    of = np.arange(groups) % kinds
+    dg, du = (up(synth.quant_matrix(quant, kinds * ffn, hidden, rng).reshape(kinds, -1)[of]) for _ in range(2))
+    dd = up(synth.quant_matrix(quant, kinds * hidden, ffn, rng).reshape(kinds, -1)[of])
+    gs, ds = ffn * rbs[0], hidden * rbs[1]
+    bank = K.ExpertBank(dg.data_ptr(), du.data_ptr(), dd.data_ptr(), None, None, None, gs, gs, ds, 0, 0, 0)
+    shared = [(dg.data_ptr() + e * gs, du.data_ptr() + e * gs, dd.data_ptr() + e * ds) for e in range(E, groups)]
+    ids = torch.from_numpy(rng.integers(0, E, (T, k)).astype(np.int32)).to(dev)
+    gptrs, starts = zeros_u8(groups * 48), torch.zeros(groups + 1, dtype=torch.int32, device=dev)
+    pairs, sw, xq = torch.zeros(n, dtype=torch.int32, device=dev), zeros_f32((T, slots)), zeros_u8(T * 2 * 292)
+    K.moe_group_ids(gptrs, starts, pairs, sw, ids, up_f32(rng.random((T, k)) + 0.1), bank, E, shared, T, k)
+    K.quantize_q8_k(xq, up_f32(rng.standard_normal((T, hidden))), hidden, T)
+    midq = up(oracle.quantize_q8_k(rng.standard_normal((n, ffn)).astype(np.float32)))
+    got = []
+    for slices in ([(0, groups)], [(0, 1024), (1024, groups)]):
+        mid, part = zeros_f32((n, ffn)), zeros_f32((n, hidden))
+        for a, b in slices:
+            K.moe_pair_swiglu_grouped(mid, gptrs[48 * a:], starts[a:], pairs, sw, xq, hidden, ffn, slots, b - a, rbs[0],
+                                      quant, 0)
+            K.moe_down_grouped(part, gptrs[48 * a:], starts[a:], pairs, midq, ffn, hidden, slots, b - a, rbs[1], quant)
+        got.append((down(mid), down(part)))
+    for one, two in zip(*got):
+        assert one.any(1).all() and np.array_equal(one.view(np.uint32), two.view(np.uint32))
