@@ -311,15 +311,15 @@ int pulsar_moe_group_csr(void *gptrs, void *starts, void *pairs, const void *ptr
  * n_group = n_expert + n_shared and n_used = k_used + n_shared. Those have a fast
  * path for long groups up to n_group = 1024: behind 1024 experts, call them once on
  * the first 1024 groups and once on the shared slots' (gptrs and starts + 1024,
- * n_group = n_shared, the same pairs), which writes the same rows. 8192 tokens of
- * 8 + 1 slots, 2048 x 512 values: gate / up 0.9 ms in two calls, 12.4 in one for
- * Q4_K, 81 for IQ4_XS. selected int32
- * [n_tok][k_used]; ids outside [0, n_expert) get no pair, so the caller zeroes
- * partial as for any CSR. slot_weights f32 [n_tok][k_used + n_shared], left out
- * where NULL: router_weights [n_tok][k_used], then 1 for the shared slots.
- * n_expert <= 1024, k_used + n_shared <= 16, n_shared <= 4, n_tok <= 2^28,
- * n_tok * (k_used + n_shared) < 2^31; bank and shared are host pointers read at
- * launch. An output over an input or another output is refused, but for
+ * n_group = n_shared, the same pairs), which writes the same rows, to the rounding
+ * for Q3_K and IQ4_XS, whose long groups run on another kernel. 8192 tokens of 8 +
+ * 1 slots, 2048 x 512 values: gate / up 0.9 ms in two calls, 12.4 in one for Q4_K,
+ * 81 for IQ4_XS. selected int32 [n_tok][k_used]; ids outside [0, n_expert) get no
+ * pair, so the caller zeroes partial as for any CSR. slot_weights f32 [n_tok][k_used
+ * + n_shared], left out where NULL: router_weights [n_tok][k_used], then 1 for the
+ * shared slots. n_expert <= 1024, k_used + n_shared <= 16, n_shared <= 4, n_tok <=
+ * 2^28, n_tok * (k_used + n_shared) < 2^31; bank and shared are host pointers read
+ * at launch. An output over an input or another output is refused, but for
  * slot_weights that are router_weights themselves where n_shared is 0. gptrs and
  * starts are working memory too while the call runs: two calls that may run at
  * once take buffers of their own. */

@@ -60,12 +60,10 @@ _F32 = (_lib.torch.float32, _lib.torch.uint8) if _lib.torch else ()
 _I32 = (_lib.torch.int32, _lib.torch.uint32, _lib.torch.uint8) if _lib.torch else ()
 
 
-def _room(buf, nbytes: int, op: str, what: str, device: int, types=None, other=None) -> int:
+def _room(buf, nbytes: int, op: str, what: str, device: int, types=None) -> int:
     """The device address of `buf`, which the launch uses the first nbytes
-    bytes of; a tensor has to be contiguous, that large and on the current
-    device (a raw address is the caller's word for all three). One that is not
-    of `types` goes to the list `other`, for _refuse: of a wider type it is
-    large enough, but its bytes are other numbers."""
+    bytes of; a tensor has to be contiguous, that large, on the current device
+    and of `types` (a raw address is the caller's word for all four)."""
     if buf is None or not hasattr(buf, "data_ptr"):
         return _ptr(buf)
     if buf.get_device() != device:
@@ -73,18 +71,18 @@ def _room(buf, nbytes: int, op: str, what: str, device: int, types=None, other=N
     if buf.nbytes < nbytes or not buf.is_contiguous():
         raise ValueError(f"{op}: {what} has to be contiguous and hold {nbytes} bytes")
     if types is not None and buf.dtype not in types:
-        other.append((what, "f32" if types is _F32 else "int32", buf.dtype))
+        _other_type(buf, op, what, types)
     return buf.data_ptr()
+
+
+def _other_type(buf, op: str, what: str, types) -> None:
+    """Of a wider type it is large enough, but its bytes are other numbers."""
+    raise ValueError(f"{op}: {what} has to be {'f32' if types is _F32 else 'int32'} (got {buf.dtype})")
 
 
 def _out_of_range(op: str) -> None:
     """A number that ctypes would cut to its low bits, -1 to the largest one."""
     raise ValueError(f"{op}: a size or code is out of range")
-
-
-def _refuse(op: str, other) -> None:
-    what, want, got = other[0]
-    raise ValueError(f"{op}: {what} has to be {want} (got {got})")
 
 
 def _misplaced(buf, op: str, what: str) -> None:
@@ -129,14 +127,14 @@ def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok
     block, block_bytes = BLOCK_LAYOUT.get(quant & ~QUANT_A4_OK, (1, 0))
     w_bytes = (out_dim - 1) * row_bytes + in_dim // block * block_bytes
     xq_bytes, so, sr = n_tok * -(-in_dim // 256) * 292, out_stride or out_dim, res_stride or out_dim
-    other = []
-    arrays = (_rows(out, n_tok, out_dim, so, op, "out", dev), _room(w, w_bytes, op, "w", dev),
-              _room(xq, xq_bytes, op, "xq", dev), _room(bias, 4 * out_dim, op, "bias", dev, _F32, other),
-              _rows(residual, n_tok, out_dim, sr, op, "residual", dev))
-    if other:
-        _refuse(op, other)
-    _check(_lib.load().pulsar_matmul_kq_fused(*arrays, in_dim, out_dim, n_tok, row_bytes, quant, act, out_stride,
-                                              res_stride), op)
+    _check(
+        _lib.load().pulsar_matmul_kq_fused(
+            _rows(out, n_tok, out_dim, so, op, "out", dev), _room(w, w_bytes, op, "w", dev),
+            _room(xq, xq_bytes, op, "xq", dev), _room(bias, 4 * out_dim, op, "bias", dev, _F32),
+            _rows(residual, n_tok, out_dim, sr, op, "residual", dev), in_dim, out_dim, n_tok, row_bytes, quant, act,
+            out_stride, res_stride),
+        op,
+    )
 
 
 def moe_pair_swiglu(mid, ptrs, weights, x, in_dim: int, mid_dim: int, n_used: int, n_tok: int,
@@ -213,17 +211,18 @@ def router_select_groups(selected, weights, logits, bias, n_expert: int, k_used:
     """Top-k of the experts of the topk_group best of n_group expert groups
     (a group's score: its group_top largest score + bias; formats.SCORE_*),
     the weights the winners' scores, renormalised if renorm, times weight_scale."""
-    op, dev, other = "router_select_groups", _device(), []
+    op, dev = "router_select_groups", _device()
     if (n_expert | k_used | n_group | topk_group | group_top | score | n_tok) >> 32:
         _out_of_range(op)
-    arrays = (_room(selected, 4 * n_tok * k_used, op, "selected", dev, _I32, other),
-              _room(weights, 4 * n_tok * k_used, op, "weights", dev, _F32, other),
-              _room(logits, 4 * n_tok * n_expert, op, "logits", dev, _F32, other),
-              _room(bias, 4 * n_expert, op, "bias", dev, _F32, other))
-    if other:
-        _refuse(op, other)
-    _check(_lib.load().pulsar_router_select_groups(*arrays, n_expert, k_used, n_group, topk_group, group_top, score,
-                                                   int(bool(renorm)), weight_scale, n_tok), op)
+    _check(
+        _lib.load().pulsar_router_select_groups(
+            _room(selected, 4 * n_tok * k_used, op, "selected", dev, _I32),
+            _room(weights, 4 * n_tok * k_used, op, "weights", dev, _F32),
+            _room(logits, 4 * n_tok * n_expert, op, "logits", dev, _F32),
+            _room(bias, 4 * n_expert, op, "bias", dev, _F32), n_expert, k_used, n_group, topk_group, group_top, score,
+            int(bool(renorm)), weight_scale, n_tok),
+        op,
+    )
 
 
 def matmul_f32(out, w, x, in_dim: int, out_dim: int, n_tok: int) -> None:
@@ -281,20 +280,21 @@ def moe_group_ids(gptrs, starts, pairs, slot_weights, selected, router_weights, 
     (gptrs and starts of the groups behind 1024 in the second): one leaves their
     fast path. slot_weights (None: left out) gets router_weights and the shared
     slots' ones."""
-    op, dev, other = "moe_group_ids", _device(), []
+    op, dev = "moe_group_ids", _device()
     if (n_expert | n_tok | k_used) >> 32:
         _out_of_range(op)
     arr, n_shared = _shared_array(shared)
     groups, slots = n_expert + n_shared, k_used + n_shared
-    arrays = (_room(gptrs, EXPERT_PTRS_BYTES * groups, op, "gptrs", dev),
-              _room(starts, 4 * (groups + 1), op, "starts", dev, _I32, other),
-              _room(pairs, 4 * n_tok * slots, op, "pairs", dev, _I32, other),
-              _room(slot_weights, 4 * n_tok * slots, op, "slot_weights", dev, _F32, other),
-              _room(selected, 4 * n_tok * k_used, op, "selected", dev, _I32, other),
-              _room(router_weights, 4 * n_tok * k_used, op, "router_weights", dev, _F32, other))
-    if other:
-        _refuse(op, other)
-    _check(_lib.load().pulsar_moe_group_ids(*arrays, ctypes.byref(bank), n_expert, arr, n_shared, n_tok, k_used), op)
+    gptrs = _room(gptrs, EXPERT_PTRS_BYTES * groups, op, "gptrs", dev)
+    starts = _room(starts, 4 * (groups + 1), op, "starts", dev, _I32)
+    pairs = _room(pairs, 4 * n_tok * slots, op, "pairs", dev, _I32)
+    weights = _room(slot_weights, 4 * n_tok * slots, op, "slot_weights", dev)
+    selected = _room(selected, 4 * n_tok * k_used, op, "selected", dev, _I32)
+    router_weights = _room(router_weights, 4 * n_tok * k_used, op, "router_weights", dev, _F32)
+    if hasattr(slot_weights, "data_ptr") and slot_weights.dtype not in _F32:  # behind every size
+        _other_type(slot_weights, op, "slot_weights", _F32)
+    _check(_lib.load().pulsar_moe_group_ids(gptrs, starts, pairs, weights, selected, router_weights,
+                                            ctypes.byref(bank), n_expert, arr, n_shared, n_tok, k_used), op)
 
 
 def moe_slot_sum_bias(out, partial, ptrs, weights, out_dim: int, n_used: int, n_tok: int) -> None:

@@ -8,11 +8,13 @@ import pytest
 import torch
 
 import oracle
+from pulsar_amd import formats as fm
 from pulsar_amd import kernels as K
 from pulsar_amd import synth
 from pulsar_amd.formats import QUANT_Q4_K, QUANT_Q6_K, SCORE_SIGMOID, SCORE_SOFTMAX, row_bytes
 from tests.gpu_util import assert_rows_close, down, up, up_f32, zeros_f32, zeros_u8
 from tests.test_gpu_group_ids import want_long
+from tests.test_gpu_grouped_choice import ROW16
 from tests.test_gpu_router_groups import want_route
 from tests.test_gpu_tile import rows_want
 
@@ -91,11 +93,11 @@ def test_layer(dev, T, E, k, G, kept, n_shared, empty, score):
     assert (np.abs(sums[at] - total) <= slots * 2.0**-24 * size).all()  # a rounding an addition
 
 
-@pytest.mark.parametrize("quant", [GQ, DQ])
+@pytest.mark.parametrize("quant", ROW16, ids=lambda q: fm.NAMES[q])
 def test_stages_in_slices_of_the_groups(dev, quant):
     """1024 experts and two shared slots, the grouped stages called on 1024 groups
     and on the two behind them, whose starts go on where the others' end: the rows
-    of one call on all."""
+    of one call on all, bit for bit where both calls' kernels sum alike."""
     T, E, k, n_shared, hidden, ffn = 3300, 1024, 4, 2, 512, 256
     rng = np.random.default_rng(5)
     slots, groups, n = k + n_shared, E + n_shared, T * (k + n_shared)
