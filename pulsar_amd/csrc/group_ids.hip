@@ -13,7 +13,9 @@
 
 namespace pk {
 
-// v with lane `lane` replaced by x (both uniform)
+// v with lane `lane` replaced by x (both uniform); there is no builtin for it. A
+// select by the lane in its place makes the compiler do it for every strip: 301
+// tokens of 256 experts 5.0 -> 6.2 us, 2048 of 1024 9.0 -> 12.0
 __device__ int32_t write_lane(int32_t x, int32_t lane, int32_t v) __asm("llvm.amdgcn.writelane.i32");
 
 constexpr uint32_t kGidThreads = 1024, kGidWaves = kGidThreads / 64u;

@@ -12,9 +12,9 @@
 // on a rounding; equal scores go to the lower id.
 //
 // What a token costs is its order, not its bytes: 16384 tokens of 256 experts in 8
-// groups, 8 winners, take 8.6 us, 3.5 of them a launch of that many blocks, where
+// groups, 8 winners, take 8.7 us, 3.5 of them a launch of that many blocks, where
 // their logits pass at 4.8 TB/s in 3.7 us; by route_token_f64 alone, a wave a token,
-// 37.6. One token: 4.0 us; 4096 tokens of 128 experts, softmax: 3.5.
+// 37.6. One token: 3.9 us; 4096 tokens of 128 experts, softmax: 3.6.
 #include "pk_route.h"
 
 namespace pk {
