@@ -7,8 +7,8 @@
 // Where a kernel has registers for what an epilogue adds (Term), it fetches it ahead
 // of the sum it belongs to, and ahead of the loads that the sum waits for: behind a
 // branch that leaves a fetch out, the compiler can only count what was requested
-// after it. matvec_kernel and ksplit_kernel do; the kernel of rows of more than 128
-// lanes' units, the 16-row kernel and the wide tile fetch at their end.
+// after it. matvec_kernel and ksplit_kernel do; matvec_wide_kernel (rows of more than
+// 32768 values), the 16-row kernel and the wide tile fetch at their end.
 #pragma once
 
 #include "pk_common.h"
@@ -26,9 +26,9 @@ PK_DEV float exp_near(float x) {
     return __builtin_amdgcn_exp2f(p) *
            __builtin_fmaf(__builtin_amdgcn_fmed3f(lo, -0.5f, 0.5f), 0.693147181f, 1.0f);
 }
-// 1 / (1 + e^-x) within 4 units: e^-x's 2, the sum's half, the reciprocal
-// instruction's 1. expf and a division were within 2 and cost a 14336 x
-// 4096 product of 512 tokens with SiLU 3 of 93 us; a dot before it is off by more
+// 1 / (1 + e^-x) within 4 units (0 below 2^-126): e^-x's 2, the sum's half, the
+// reciprocal instruction's 1. expf and a division are within 2, and cost a product
+// of 14336 x 4096 with 512 tokens and SiLU 3 of 93 us; its dots are off by more
 PK_DEV float sigmoid_near(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_near(-x)); }
 
 struct PlainOut {

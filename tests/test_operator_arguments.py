@@ -76,6 +76,19 @@ def test_sound_arguments_reach_the_library(call):
         call()
 
 
+def test_raw_bytes_reach_the_library():
+    """A buffer of bytes stands for any array but the product's rows."""
+    if torch.cuda.is_available():
+        pytest.skip("these addresses are nobody's")
+    raw = lambda n: Placed((n,), torch.uint8)  # noqa: E731
+    for call in (lambda: route(selected=raw(4 * T * N), weights=raw(4 * T * N), logits=raw(4 * T * E), bias=raw(4 * E)),
+                 lambda: group(gptrs=raw(48 * E), starts=raw(4 * E + 4), pairs=raw(4 * T * N), selected=raw(4 * T * N),
+                               slot_weights=raw(4 * T * N), router_weights=raw(4 * T * N)),
+                 lambda: product(bias=raw(4 * ROWS))):
+        with pytest.raises(K.KernelError):
+            call()
+
+
 WIDE = [(route, "selected", (T, N), torch.int64), (route, "selected", (T, N), F32),
         (route, "weights", (T, N), torch.float64), (route, "weights", (T, 2 * N), torch.float16),
         (route, "logits", (T, E), torch.float64), (route, "logits", (T, 2 * E), torch.bfloat16),
