@@ -72,6 +72,16 @@ extern "C" {
 #define PULSAR_SCORE_SIGMOID 0u
 #define PULSAR_SCORE_SOFTMAX 1u
 
+/* element types of the rows that pulsar_rms_norm_q8, pulsar_quantize_i8 and
+ * pulsar_matmul_i8 read or write (every other call's rows are f32) */
+#define PULSAR_TYPE_F32  0u
+#define PULSAR_TYPE_F16  1u
+#define PULSAR_TYPE_BF16 2u
+
+/* 8-bit rows that pulsar_rms_norm_q8 writes */
+#define PULSAR_ROWS_Q8_K 0u /* q8_K blocks */
+#define PULSAR_ROWS_I8   1u /* int8 values, one f32 scale a row */
+
 #define PULSAR_QK_K 256u
 
 /* q8_K activation block (pulsar_kernels.cu:1492-1496; lane Q8KRow,
@@ -121,6 +131,64 @@ int pulsar_quantize_q8_K(void *out, const void *x, uint32_t in_dim, uint32_t n_r
 int pulsar_matmul_kq(void *out, const void *w, const void *xq, uint32_t in_dim,
                      uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes,
                      uint32_t quant);
+
+/* ---- 8-bit rows with a scale each, and what a layer makes them of (no reference
+ * counterpart: the reference runs its norms in kernels of their own and quantizes
+ * their f32 rows) ----
+ *
+ * Codes of 8 bits, in all of these: of values v with the largest size A = max |v|
+ * (of the row, or of a q8_K block), q = 127 v / A to the nearest integer, halves away
+ * from 0, decided as it stands in 64 bits (an argument nearer than 2^-40 to a half
+ * counts as on it); the scale is A / 127, rounded to f32. A row of zeros has codes and
+ * scale 0. Where a row (block) holds a NaN its scale is NaN, where it holds an infinity
+ * the scale is infinite (in the norm, whose root is infinite then, NaN); the codes of
+ * what is not finite are 0. Strides count elements (bytes in int8 rows), 0 stands for
+ * packed rows; what lies between rows is left as it is. */
+
+/* s = x + residual (NULL: x), rounded to `type`; y = s * gain / sqrt(mean(s^2) + eps)
+ * and its 8-bit form, in one pass:
+ *   sum       s, rows of `type` (NULL: left out); may be x or residual itself, at the
+ *             same stride
+ *   y         packed rows of `type` (NULL: left out)
+ *   q         format PULSAR_ROWS_Q8_K: q8_K [n_rows][ceil(dim / 256)], as
+ *             pulsar_matmul_kq and the routed stages read them, values past dim 0;
+ *             scales NULL, q_stride 0. PULSAR_ROWS_I8: int8 rows q_stride apart, scales
+ *             f32 [n_rows], as pulsar_matmul_i8 reads them. NULL: left out
+ * gain f32 [dim]. The codes are those of s * gain, which the root does not change, so
+ * they are not off by y's rounding: pulsar_quantize_q8_K of y, which decides in f32,
+ * gives another code for about one value in 10^5, by 1. Sums of squares are kept in 64
+ * bits and do not overflow. A row of zeros gives zeros with eps 0 too; eps >= 0. y or q
+ * has to be there. dim <= 2^24, n_rows < 2^31, strides < 2^32. Outputs over an input or another
+ * output are refused, but for sum as above. */
+int pulsar_rms_norm_q8(void *q, void *scales, void *y, void *sum, const void *x,
+                       const void *residual, const void *gain, uint32_t dim, uint32_t n_rows,
+                       float eps, uint32_t type, uint32_t format, uint64_t x_stride,
+                       uint64_t res_stride, uint64_t sum_stride, uint64_t q_stride);
+
+/* Rows of `type` to int8 rows with a scale each (f32 [n_rows]): of v = x, or where up
+ * is given of v = glu(x, up, act_op), the gated combine of pulsar_moe_pair_swiglu in 64
+ * bits (SWIGLU_OAI's alpha: 1.702). up NULL: act_op 0. gate and up may be columns of one
+ * array. dim <= 2^24, n_rows < 2^31, strides < 2^32. q or scales over an input or one
+ * another are refused. */
+int pulsar_quantize_i8(void *q, void *scales, const void *x, const void *up, uint32_t dim,
+                       uint32_t n_rows, uint32_t act_op, uint32_t type, uint64_t x_stride,
+                       uint64_t up_stride, uint64_t q_stride);
+
+/* out[t][r] = act(x_scales[t] w_scales[r] sum_i x[t][i] w[r][i] + bias[r]) + residual[t][r]
+ * int8 x [n_tok] and w [out_dim] rows of in_dim values, x_stride and w_stride bytes apart;
+ * f32 x_scales [n_tok], w_scales [out_dim], bias [out_dim] (NULL: none); residual (NULL:
+ * none) and out rows of `type`, res_stride and out_stride elements apart; act: a
+ * PULSAR_EPI_* code. The sums are exact in 32 bits (in_dim <= 131071: 2^14 a product);
+ * sum, times the token's scale, times the channel's: a rounding to f32 each, as for bias,
+ * activation and residual; one to `type` at the end. residual may be out itself, at the
+ * same stride; any other overlap of out with an operand is refused. x_stride and w_stride
+ * <= 2^23, out_stride and res_stride < 2^32. Rows on a 16-byte boundary (base and stride) run
+ * fastest. */
+int pulsar_matmul_i8(void *out, const void *w, const void *w_scales, const void *x,
+                     const void *x_scales, const void *bias, const void *residual,
+                     uint32_t in_dim, uint32_t out_dim, uint32_t n_tok, uint32_t act,
+                     uint32_t type, uint64_t w_stride, uint64_t x_stride, uint64_t out_stride,
+                     uint64_t res_stride);
 
 /* pulsar_matmul_kq with its epilogue in the same launch (no reference
  * counterpart: the reference runs the bias, the activation and the residual

@@ -33,6 +33,9 @@ ACT_SWIGLU_OAI = 2
 # expert groups (PULSAR_SCORE_*) in include/pulsar_moe.h
 EPI_NONE, EPI_SILU, EPI_GELU, EPI_RELU, EPI_SIGMOID = range(5)
 SCORE_SIGMOID, SCORE_SOFTMAX = range(2)
+# element types of rows (PULSAR_TYPE_*) and 8-bit rows of the norm (PULSAR_ROWS_*)
+TYPE_F32, TYPE_F16, TYPE_BF16 = range(3)
+ROWS_Q8_K, ROWS_I8 = range(2)
 
 QK_K = 256
 Q8_K_BLOCK_BYTES = 292  # f32 d, i8 qs[256], i16 bsums[16]

@@ -16,7 +16,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from .formats import BLOCK_LAYOUT, EXPERT_PTRS_BYTES, QUANT_A4_OK
+from .formats import BLOCK_LAYOUT, EXPERT_PTRS_BYTES, QUANT_A4_OK, ROWS_Q8_K
 
 
 class KernelError(RuntimeError):
@@ -96,24 +96,36 @@ def _device() -> int:
     return cuda.current_device() if cuda.is_initialized() else -2
 
 
-def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str, device: int) -> int:
-    """The device address of n_rows rows of dim floats, `stride` floats apart.
-    A tensor may be a view of columns of a wider array: it has to be f32 [..,
+# element types of rows, by their PULSAR_TYPE_* code, and of int8 rows
+_TYPES = (_lib.torch.float32, _lib.torch.float16, _lib.torch.bfloat16) if _lib.torch else (None,) * 3
+_I8 = _lib.torch.int8 if _lib.torch else None
+_TYPE_NAMES = dict(zip((*_TYPES, _I8), ("f32", "f16", "bf16", "int8")))
+
+
+def _rows(buf, n_rows: int, dim: int, stride: int, op: str, what: str, device: int, dtype=_TYPES[0]) -> int:
+    """The device address of n_rows rows of dim values, `stride` values apart.
+    A tensor may be a view of columns of a wider array: it has to be of dtype, [..,
     dim] with that stride, or contiguous and large enough."""
     if buf is None or not hasattr(buf, "data_ptr"):
         return _ptr(buf)
     if buf.get_device() != device:
         _misplaced(buf, op, what)
-    if buf.dtype != _lib.torch.float32:
-        raise ValueError(f"{op}: {what} has to be f32 (got {buf.dtype})")
+    if buf.dtype != dtype:
+        raise ValueError(f"{op}: {what} has to be {_TYPE_NAMES[dtype]} (got {buf.dtype})")
     if buf.is_contiguous():
         ok = buf.numel() >= (n_rows - 1) * stride + dim
     else:
         ok = (buf.dim() == 2 and buf.shape[0] >= n_rows and buf.shape[1] >= dim and buf.stride(1) == 1
               and buf.stride(0) == stride)
     if not ok:
-        raise ValueError(f"{op}: {what} has to hold {n_rows} rows of {dim} f32 values {stride} apart")
+        raise ValueError(f"{op}: {what} has to hold {n_rows} rows of {dim} {_TYPE_NAMES[dtype]} values {stride} apart")
     return buf.data_ptr()
+
+
+def _type(code: int, op: str):
+    if not 0 <= code < len(_TYPES):
+        _out_of_range(op)
+    return _TYPES[code]
 
 
 def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok: int, row_bytes: int, quant: int,
@@ -133,6 +145,53 @@ def matmul_kq_fused(out, w, xq, bias, residual, in_dim: int, out_dim: int, n_tok
             _room(xq, xq_bytes, op, "xq", dev), _room(bias, 4 * out_dim, op, "bias", dev, _F32),
             _rows(residual, n_tok, out_dim, sr, op, "residual", dev), in_dim, out_dim, n_tok, row_bytes, quant, act,
             out_stride, res_stride),
+        op,
+    )
+
+
+def rms_norm_q8(q, scales, y, sum_out, x, residual, gain, dim: int, n_rows: int, eps: float, type: int = 0,
+                fmt: int = ROWS_Q8_K, x_stride: int = 0, res_stride: int = 0, sum_stride: int = 0,
+                q_stride: int = 0) -> None:
+    """sum_out = x + residual, y = its root-mean-square norm times gain, and y in 8
+    bits, in one pass: q8_K blocks in q (formats.ROWS_Q8_K, scales None) or int8 rows
+    with a scale each (formats.ROWS_I8). residual, sum_out, y and q may be None (y or q
+    has to be there), sum_out may be x or residual itself. Rows are of a formats.TYPE_*
+    code, gain f32; strides in elements, 0 for packed rows."""
+    op, dev = "rms_norm_q8", _device()
+    if (dim | n_rows | type | fmt) >> 32 or (x_stride | res_stride | sum_stride | q_stride) >> 64:
+        _out_of_range(op)
+    t = _type(type, op)
+    if fmt == ROWS_Q8_K:
+        codes = _room(q, n_rows * -(-dim // 256) * 292, op, "q", dev)
+    else:
+        codes = _rows(q, n_rows, dim, q_stride or dim, op, "q", dev, _I8)
+    _check(
+        _lib.load().pulsar_rms_norm_q8(
+            codes, _room(scales, 4 * n_rows, op, "scales", dev, _F32), _rows(y, n_rows, dim, dim, op, "y", dev, t),
+            _rows(sum_out, n_rows, dim, sum_stride or dim, op, "sum_out", dev, t),
+            _rows(x, n_rows, dim, x_stride or dim, op, "x", dev, t),
+            _rows(residual, n_rows, dim, res_stride or dim, op, "residual", dev, t),
+            _room(gain, 4 * dim, op, "gain", dev, _F32), dim, n_rows, eps, type, fmt, x_stride, res_stride, sum_stride,
+            q_stride),
+        op,
+    )
+
+
+def quantize_i8(q, scales, x, up, dim: int, n_rows: int, act_op: int = 0, type: int = 0, x_stride: int = 0,
+                up_stride: int = 0, q_stride: int = 0) -> None:
+    """Rows of a formats.TYPE_* code to int8 rows with an f32 scale each: x as it is
+    (up None), or glu(x, up, act_op) (formats.ACT_*). Strides in elements, 0 for packed
+    rows."""
+    op, dev = "quantize_i8", _device()
+    if (dim | n_rows | act_op | type) >> 32 or (x_stride | up_stride | q_stride) >> 64:
+        _out_of_range(op)
+    t = _type(type, op)
+    _check(
+        _lib.load().pulsar_quantize_i8(
+            _rows(q, n_rows, dim, q_stride or dim, op, "q", dev, _I8), _room(scales, 4 * n_rows, op, "scales", dev, _F32),
+            _rows(x, n_rows, dim, x_stride or dim, op, "x", dev, t),
+            _rows(up, n_rows, dim, up_stride or dim, op, "up", dev, t), dim, n_rows, act_op, type, x_stride, up_stride,
+            q_stride),
         op,
     )
 
