@@ -55,6 +55,7 @@ SIGNATURES = {
     "pulsar_moe_group_ids": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _u32, _u32, _u32],
     "pulsar_rms_norm_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _f32, _u32, _u32, _u64, _u64, _u64, _u64],
     "pulsar_quantize_i8": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u64, _u64, _u64],
+    "pulsar_matmul_i8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u64, _u64, _u64, _u64],
     "pulsar_moe_selftest": [],
     "pulsar_router_selftest": [],
 }

@@ -19,7 +19,8 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libpulsar_moe.so"
 SOURCES = ["q8k.hip", "matvec.hip", "mmq.hip", "tile.hip", "ksplit.hip", "tile_moe.hip", "moe.hip", "router.hip",
-           "router_groups.hip", "route.hip", "group_ids.hip", "fused.hip", "rows8.hip", "selftest.hip"]
+           "router_groups.hip", "route.hip", "group_ids.hip", "fused.hip", "rows8.hip", "product_i8.hip",
+           "selftest.hip"]
 ARCH = os.environ.get("PULSAR_OFFLOAD_ARCH", "gfx950")
 
 # -ffp-contract=off: the compiler fuses no a*b+c on its own, so fp32

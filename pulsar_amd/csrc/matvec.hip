@@ -265,21 +265,6 @@ static int dense_product(const char *what, void *out, const void *w, const void 
 #undef PK_MVQ
 }
 
-// Whether the rows of out may be written while those of residual are read:
-// the same rows (an element is read before it is written), apart, or columns
-// of one wider array that share no float.
-static bool rows_allow(const void *out, uint64_t out_stride, const void *res, uint64_t res_stride, uint32_t dim,
-                       uint32_t n_tok) {
-    if (out == res && out_stride == res_stride) return true;
-    auto bytes = [&](uint64_t stride) { return 4 * ((u128)(n_tok - 1u) * stride + dim); };
-    if (!overlap(out, bytes(out_stride), res, bytes(res_stride))) return true;
-    if (out_stride != res_stride) return false;
-    const u128 row = 4 * (u128)out_stride, width = 4 * (u128)dim;
-    const uint64_t a = (uint64_t)(uintptr_t)out, b = (uint64_t)(uintptr_t)res;
-    const u128 apart = b >= a ? (b - a) % row : (row - (a - b) % row) % row;
-    return apart >= width && apart + width <= row;
-}
-
 }  // namespace pk
 
 // pulsar_kernels.cu:4895-4906 contract: in_dim a multiple of 256, nonzero
@@ -309,7 +294,7 @@ extern "C" int pulsar_matmul_kq_fused(void *out, const void *w, const void *xq, 
         return pk::reject("matmul_kq_fused");
     const pk::u128 out_bytes = 4 * ((pk::u128)(n_tok - 1u) * out_stride + out_dim);
     const pk::u128 xq_bytes = (pk::u128)n_tok * (in_dim / 256u) * 292u;
-    if (out_bytes >> 62 || (residual && !pk::rows_allow(out, out_stride, residual, res_stride, out_dim, n_tok)) ||
+    if (out_bytes >> 62 || (residual && !pk::rows_allow(out, out_stride, residual, res_stride, out_dim, n_tok, 4u)) ||
         pk::overlap(out, out_bytes, xq, xq_bytes) || pk::overlap(out, out_bytes, w, (pk::u128)out_dim * row_bytes) ||
         (bias && pk::overlap(out, out_bytes, bias, 4 * (pk::u128)out_dim)))
         return pk::reject("matmul_kq_fused (overlap)");

@@ -41,6 +41,21 @@ static inline bool overlap(const void *a, u128 an, const void *b, u128 bn) {
     return (u128)(uintptr_t)a < (uintptr_t)b + bn && (u128)(uintptr_t)b < (uintptr_t)a + an;
 }
 
+// Whether the rows of out (dim values of `size` bytes) may be written while those of
+// residual are read: the same rows (an element is read before it is written), apart, or
+// columns of one wider array that share no value.
+static inline bool rows_allow(const void *out, uint64_t out_stride, const void *res, uint64_t res_stride, uint32_t dim,
+                              uint32_t n_rows, uint32_t size) {
+    if (out == res && out_stride == res_stride) return true;
+    auto bytes = [&](uint64_t stride) { return size * ((u128)(n_rows - 1u) * stride + dim); };
+    if (!overlap(out, bytes(out_stride), res, bytes(res_stride))) return true;
+    if (out_stride != res_stride) return false;
+    const u128 row = size * (u128)out_stride, width = size * (u128)dim;
+    const uint64_t a = (uint64_t)(uintptr_t)out, b = (uint64_t)(uintptr_t)res;
+    const u128 apart = b >= a ? (b - a) % row : (row - (a - b) % row) % row;
+    return apart >= width && apart + width <= row;
+}
+
 // A pointer read from memory (expert tables) is generic to the compiler;
 // this marks it as global memory so loads through it are global loads.
 PK_DEV const uint8_t *as_global(const void *p) {

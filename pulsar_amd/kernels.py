@@ -196,6 +196,29 @@ def quantize_i8(q, scales, x, up, dim: int, n_rows: int, act_op: int = 0, type: 
     )
 
 
+def matmul_i8(out, w, w_scales, x, x_scales, bias, residual, in_dim: int, out_dim: int, n_tok: int, act: int = 0,
+              type: int = 0, w_stride: int = 0, x_stride: int = 0, out_stride: int = 0, res_stride: int = 0) -> None:
+    """out[t] = act(x_scales[t] * w_scales * (w x_t) + bias) + residual[t] of int8 rows,
+    sums exact (formats.EPI_* codes; bias and residual may be None, residual may be out
+    itself). out and residual are of a formats.TYPE_* code, scales and bias f32; strides
+    in elements, 0 for packed rows."""
+    op, dev = "matmul_i8", _device()
+    if (in_dim | out_dim | n_tok | act | type) >> 32 or (w_stride | x_stride | out_stride | res_stride) >> 64:
+        _out_of_range(op)
+    t = _type(type, op)
+    _check(
+        _lib.load().pulsar_matmul_i8(
+            _rows(out, n_tok, out_dim, out_stride or out_dim, op, "out", dev, t),
+            _rows(w, out_dim, in_dim, w_stride or in_dim, op, "w", dev, _I8),
+            _room(w_scales, 4 * out_dim, op, "w_scales", dev, _F32),
+            _rows(x, n_tok, in_dim, x_stride or in_dim, op, "x", dev, _I8),
+            _room(x_scales, 4 * n_tok, op, "x_scales", dev, _F32), _room(bias, 4 * out_dim, op, "bias", dev, _F32),
+            _rows(residual, n_tok, out_dim, res_stride or out_dim, op, "residual", dev, t), in_dim, out_dim, n_tok, act,
+            type, w_stride, x_stride, out_stride, res_stride),
+        op,
+    )
+
+
 def moe_pair_swiglu(mid, ptrs, weights, x, in_dim: int, mid_dim: int, n_used: int, n_tok: int,
                     row_bytes: int, quant: int, act_op: int) -> None:
     _check(
