@@ -20,7 +20,7 @@ BUILD = PKG / "_build"
 LIB = PKG / "libpulsar_moe.so"
 SOURCES = ["q8k.hip", "matvec.hip", "mmq.hip", "tile.hip", "ksplit.hip", "tile_moe.hip", "moe.hip", "router.hip",
            "router_groups.hip", "route.hip", "group_ids.hip", "fused.hip", "rows8.hip", "product_i8.hip",
-           "selftest.hip"]
+           "product_i8_f32.hip", "product_i8_f16.hip", "product_i8_bf16.hip", "selftest.hip"]
 ARCH = os.environ.get("PULSAR_OFFLOAD_ARCH", "gfx950")
 
 # -ffp-contract=off: the compiler fuses no a*b+c on its own, so fp32

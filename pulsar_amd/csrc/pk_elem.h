@@ -30,14 +30,20 @@ struct Elem<PULSAR_TYPE_BF16> {
 static inline uint32_t elem_bytes(uint32_t type) { return type == PULSAR_TYPE_F32 ? 4u : 2u; }
 
 // Values p[0 .. 3], of which the first n (4: all, one load) are there; 0 for the others.
-// Rows may start at any element: global loads and stores take any alignment.
+// Rows may start at any element: global loads and stores take any alignment. Single
+// values are volatile so that the compiler leaves them apart from the four: where it
+// joins the last of either in one store, lanes with four values write their third twice
+// (seen behind a branch that is uniform on one side).
 template <uint32_t TYPE>
 PK_DEV void load_row4(const typename Elem<TYPE>::raw *p, uint32_t n, float (&v)[4]) {
     typename Elem<TYPE>::raw w[4] = {};
     if (n >= 4u)
         __builtin_memcpy(w, p, sizeof(w));
-    else
-        for (uint32_t j = 0; j < n; j++) w[j] = p[j];
+    else {
+#pragma unroll
+        for (uint32_t j = 0; j < 3u; j++)
+            if (j < n) w[j] = *(const volatile PK_GLOBAL typename Elem<TYPE>::raw *)(p + j);
+    }
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = Elem<TYPE>::up(w[j]);
 }
@@ -45,8 +51,11 @@ template <uint32_t TYPE>
 PK_DEV void store_row4(typename Elem<TYPE>::raw *p, uint32_t n, const typename Elem<TYPE>::raw (&w)[4]) {
     if (n >= 4u)
         __builtin_memcpy(p, w, sizeof(w));
-    else
-        for (uint32_t j = 0; j < n; j++) p[j] = w[j];
+    else {
+#pragma unroll
+        for (uint32_t j = 0; j < 3u; j++)
+            if (j < n) *(volatile PK_GLOBAL typename Elem<TYPE>::raw *)(p + j) = w[j];
+    }
 }
 
 // ------------------------------------------------- 8-bit codes of 64-bit values --

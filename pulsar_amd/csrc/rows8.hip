@@ -48,8 +48,11 @@ PK_DEV uint32_t codes4(const double (&v)[4], double factor, int32_t &sum) {
 PK_DEV void store_codes(uint8_t *p, uint32_t n, uint32_t packed) {
     if (n >= 4u)
         __builtin_memcpy(p, &packed, 4);
-    else
-        for (uint32_t j = 0; j < n; j++) p[j] = (uint8_t)(packed >> (8 * j));
+    else {
+#pragma unroll
+        for (uint32_t j = 0; j < 3u; j++)
+            if (j < n) *(volatile PK_GLOBAL uint8_t *)(p + j) = (uint8_t)(packed >> (8 * j));
+    }
 }
 
 // ------------------------------------------------------------------ norm --
