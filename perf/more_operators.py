@@ -192,6 +192,17 @@ def _product(s):
 
 # -------------------------------------------------------------------- run --
 
+def _values(s, codes, scales):
+    """The codes' values, computed on the stream that the calls go to: on torch's
+    own each pass would change streams twice, and wait for it."""
+    from pulsar_amd import runtime
+
+    if "stream" not in s:
+        s["stream"] = torch.cuda.ExternalStream(runtime.STREAM_PER_THREAD)
+    with torch.cuda.stream(s["stream"]):
+        return torch.mul(codes, scales, out=s["values"])
+
+
 def _call(s):
     from pulsar_amd import kernels as K
 
@@ -202,16 +213,16 @@ def _call(s):
         return s["out"]
     if c["op"] == "quant":
         K.quantize_i8(s["q"], s["scales"], s["x"], s["up"], c["dim"], c["rows"], GLUS[c["glu"]], kind)
-        return {"values": torch.mul(s["q"], s["scales"][:, None], out=s["values"])}
+        return {"values": _values(s, s["q"], s["scales"][:, None])}
     got = {k: s[k] for k in ("sum", "y") if s[k] is not None}
     if c["out"] == "i8":
         K.rms_norm_q8(s["q"], s["scales"], s["y"], s["sum"], s["x"], s["residual"], s["gain"], c["dim"], c["rows"], EPS,
                       kind, 1)
-        got["values"] = torch.mul(s["q"], s["scales"][:, None], out=s["values"])
+        got["values"] = _values(s, s["q"], s["scales"][:, None])
         return got
     b = s["blocks"]
     K.rms_norm_q8(b, None, s["y"], s["sum"], s["x"], s["residual"], s["gain"], c["dim"], c["rows"], EPS, kind, 0)
-    got["values"] = torch.mul(b[..., 4:260].view(torch.int8), b[..., :4].view(torch.float32), out=s["values"])
+    got["values"] = _values(s, b[..., 4:260].view(torch.int8), b[..., :4].view(torch.float32))
     got["sums"] = b[..., 260:].view(torch.int16)
     return got
 
