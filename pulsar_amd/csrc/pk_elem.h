@@ -29,33 +29,42 @@ struct Elem<PULSAR_TYPE_BF16> {
 
 static inline uint32_t elem_bytes(uint32_t type) { return type == PULSAR_TYPE_F32 ? 4u : 2u; }
 
-// Values p[0 .. 3], of which the first n (4: all, one load) are there; 0 for the others.
-// Rows may start at any element: global loads and stores take any alignment. Single
-// values are volatile so that the compiler leaves them apart from the four: where it
-// joins the last of either in one store, lanes with four values write their third twice
+// Values p[0 .. V - 1], of which the first n (V and more: all, one load) are there; 0 for
+// the others. Rows may start at any element: global loads and stores take any alignment.
+// Single values are volatile so that the compiler leaves them apart from the whole: where
+// it joins the last of either in one store, lanes that write all of them write one twice
 // (seen behind a branch that is uniform on one side).
-template <uint32_t TYPE>
-PK_DEV void load_row4(const typename Elem<TYPE>::raw *p, uint32_t n, float (&v)[4]) {
-    typename Elem<TYPE>::raw w[4] = {};
-    if (n >= 4u)
+template <uint32_t TYPE, uint32_t V>
+PK_DEV void load_row(const typename Elem<TYPE>::raw *p, uint32_t n, float (&v)[V]) {
+    typedef typename Elem<TYPE>::raw raw;
+    raw w[V] = {};
+    if (n >= V)
         __builtin_memcpy(w, p, sizeof(w));
     else {
 #pragma unroll
-        for (uint32_t j = 0; j < 3u; j++)
-            if (j < n) w[j] = *(const volatile PK_GLOBAL typename Elem<TYPE>::raw *)(p + j);
+        for (uint32_t j = 0; j + 1u < V; j++)
+            if (j < n) w[j] = *(const volatile PK_GLOBAL raw *)(p + j);
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = Elem<TYPE>::up(w[j]);
+    for (uint32_t j = 0; j < V; j++) v[j] = Elem<TYPE>::up(w[j]);
 }
-template <uint32_t TYPE>
-PK_DEV void store_row4(typename Elem<TYPE>::raw *p, uint32_t n, const typename Elem<TYPE>::raw (&w)[4]) {
-    if (n >= 4u)
+template <typename raw, uint32_t V>
+PK_DEV void store_row(raw *p, uint32_t n, const raw (&w)[V]) {
+    if (n >= V)
         __builtin_memcpy(p, w, sizeof(w));
     else {
 #pragma unroll
-        for (uint32_t j = 0; j < 3u; j++)
-            if (j < n) *(volatile PK_GLOBAL typename Elem<TYPE>::raw *)(p + j) = w[j];
+        for (uint32_t j = 0; j + 1u < V; j++)
+            if (j < n) *(volatile PK_GLOBAL raw *)(p + j) = w[j];
     }
+}
+template <uint32_t TYPE>
+PK_DEV void load_row4(const typename Elem<TYPE>::raw *p, uint32_t n, float (&v)[4]) {
+    load_row<TYPE, 4>(p, n, v);
+}
+template <uint32_t TYPE>
+PK_DEV void store_row4(typename Elem<TYPE>::raw *p, uint32_t n, const typename Elem<TYPE>::raw (&w)[4]) {
+    store_row(p, n, w);
 }
 
 // ------------------------------------------------- 8-bit codes of 64-bit values --
@@ -71,10 +80,11 @@ PK_DEV uint64_t wave_step64(uint64_t v, F &&lane32) {
 PK_DEV uint64_t partner64(uint64_t v, uint32_t s) {
     return wave_step64(v, [&](int32_t w) { return partner(w, s); });
 }
-// Largest of the wave's, in every lane
-PK_DEV uint64_t wave_max64(uint64_t v) {
+// Largest of aligned groups of G lanes, in every lane
+template <uint32_t G>
+PK_DEV uint64_t group_max64(uint64_t v) {
 #pragma unroll
-    for (uint32_t s = 1; s < 64; s <<= 1) v = max_bits(v, partner64(v, s));
+    for (uint32_t s = 1; s < G; s <<= 1) v = max_bits(v, partner64(v, s));
     return v;
 }
 PK_DEV double wave_sum64(double v) {

@@ -2,13 +2,17 @@
 // (pulsar_rms_norm_q8) and the quantizer behind a gated combine
 // (pulsar_quantize_i8).
 //
-// A row is one block's: lane l of a wave holds values 4 l .. 4 l + 3 of a chunk of 256
-// (a q8_K block), a wave NB chunks, so that the row is read once, stays in registers as
-// 64-bit products and is written once. The norm needs one exchange between the waves: its root
+// A row is one block's: a lane holds 16 bytes of a chunk (a q8_K block of f32 values, two
+// of 16-bit ones), a wave up to four chunks, so that the row is read once, stays in
+// registers and is written once. The norm needs one exchange between the waves: its root
 // divides every value of the row alike, so codes and the largest size are those of s *
-// gain, known without it. 64 bits cost no time that the bytes do not: a value is 10 to 13
-// bytes of traffic and about 10 operations at the rate of f32's.
+// gain, known without it. Sums, products and codes in 64 bits cost about what the bytes
+// do: a value is 5 to 17 bytes of traffic and some 20 operations, most of them at the rate
+// of f32's. Measured (GB/s of what has to move): norm of 8192 rows of 4096 bf16 values to
+// int8 55 us (4270), to q8_K with y 69 (4440), of 2048 rows of f32 32 (4490), quantized as
+// they are 19 (5300).
 #include "pk_elem.h"
+#include "pk_epilogue.h"
 
 namespace pk {
 
@@ -33,26 +37,28 @@ PK_DEV void block_stats(RowStats &lds, double &sum, uint64_t &top) {
     }
 }
 
-// The lane's 4 values as int8 codes, packed, and the sum of the codes
-PK_DEV uint32_t codes4(const double (&v)[4], double factor, int32_t &sum) {
-    uint32_t packed = 0;
-    sum = 0;
+// A lane's values of a chunk: 16 bytes of the rows' type. A chunk is 64 lanes' worth: one
+// q8_K block of f32 values, two of 16-bit ones
+template <uint32_t TYPE>
+constexpr uint32_t kLane = TYPE == PULSAR_TYPE_F32 ? 4u : 8u;
+
+// The lane's values as int8 codes, packed, and the sum of the codes
+template <uint32_t V>
+PK_DEV int32_t codes_of(const double (&v)[V], double factor, int8_t (&q)[V]) {
+    int32_t sum = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int32_t q = code_of(v[j], factor);
-        sum += q;
-        packed |= ((uint32_t)q & 0xffu) << (8 * j);
+    for (uint32_t j = 0; j < V; j++) {
+        const int32_t c = code_of(v[j], factor);
+        sum += c;
+        q[j] = (int8_t)c;
     }
-    return packed;
+    return sum;
 }
-PK_DEV void store_codes(uint8_t *p, uint32_t n, uint32_t packed) {
-    if (n >= 4u)
-        __builtin_memcpy(p, &packed, 4);
-    else {
-#pragma unroll
-        for (uint32_t j = 0; j < 3u; j++)
-            if (j < n) *(volatile PK_GLOBAL uint8_t *)(p + j) = (uint8_t)(packed >> (8 * j));
-    }
+
+// How many of the V values from c0 on are in the row
+template <uint32_t V>
+PK_DEV uint32_t inside(uint32_t c0, uint32_t dim) {
+    return c0 < dim ? (dim - c0 < V ? dim - c0 : V) : 0u;
 }
 
 // ------------------------------------------------------------------ norm --
@@ -70,111 +76,127 @@ struct NormArgs {
     float eps;
 };
 
-// s of 4 values: x + residual, rounded to the rows' type
-template <uint32_t TYPE>
-PK_DEV void norm_load(const NormArgs<TYPE> &a, const typename Elem<TYPE>::raw *x,
-                      const typename Elem<TYPE>::raw *res, uint32_t n, float (&s)[4]) {
-    load_row4<TYPE>(x, n, s);
+// s of V values: x + residual, rounded to the rows' type
+template <uint32_t TYPE, uint32_t V>
+PK_DEV void norm_load(const NormArgs<TYPE> &a, uint64_t row, uint32_t c0, uint32_t n, float (&s)[V]) {
+    load_row<TYPE>(a.x + row * a.x_stride + c0, n, s);
     if (!a.residual) return;
-    float r[4];
-    load_row4<TYPE>(res, n, r);
+    float r[V];
+    load_row<TYPE>(a.residual + row * a.res_stride + c0, n, r);
 #pragma unroll
-    for (int j = 0; j < 4; j++) s[j] = Elem<TYPE>::up(Elem<TYPE>::down(s[j] + r[j]));
+    for (uint32_t j = 0; j < V; j++) s[j] = Elem<TYPE>::up(Elem<TYPE>::down(s[j] + r[j]));
 }
-template <uint32_t TYPE>
-PK_DEV void norm_put_sum(typename Elem<TYPE>::raw *sum, uint32_t n, const float (&s)[4]) {
-    typename Elem<TYPE>::raw w[4];
+template <uint32_t TYPE, uint32_t V>
+PK_DEV void norm_put_sum(const NormArgs<TYPE> &a, uint64_t row, uint32_t c0, uint32_t n, const float (&s)[V]) {
+    typename Elem<TYPE>::raw w[V];
 #pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = Elem<TYPE>::down(s[j]);  // exact
-    store_row4<TYPE>(sum, n, w);
+    for (uint32_t j = 0; j < V; j++) w[j] = Elem<TYPE>::down(s[j]);  // exact
+    store_row(a.sum + row * a.sum_stride + c0, n, w);
+}
+// p = s * gain (exact), the squares of s added to ss, the largest |p|
+template <uint32_t TYPE, uint32_t V>
+PK_DEV uint64_t norm_products(const NormArgs<TYPE> &a, uint32_t c0, uint32_t n, const float (&s)[V], double (&p)[V],
+                              double &ss) {
+    float g[V];
+    load_row<PULSAR_TYPE_F32>(a.gain + c0, n, g);
+    uint64_t top = 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < V; j++) {
+        const double v = s[j];
+        ss = __builtin_fma(v, v, ss);
+        p[j] = v * (double)g[j];
+        top = max_bits(top, size_bits(p[j]));
+    }
+    return top;
 }
 PK_DEV double norm_root(double sum, uint32_t dim, float eps) {
     const double m = sum / (double)dim + (double)eps;
     return m == 0.0 ? 0.0 : 1.0 / __builtin_sqrt(m);
 }
-// y and codes of one chunk. top: the largest |p| of what shares a scale
-template <uint32_t TYPE>
-PK_DEV void norm_put(const NormArgs<TYPE> &a, uint64_t row, uint32_t b, uint32_t n, const double (&p)[4], double root,
+// y and codes of a lane's share of a chunk. top: the largest |p| of what shares a scale
+template <uint32_t TYPE, uint32_t V>
+PK_DEV void norm_put(const NormArgs<TYPE> &a, uint64_t row, uint32_t c0, uint32_t n, const double (&p)[V], double root,
                      uint64_t top, double factor) {
-    const uint32_t lane = threadIdx.x & 63u, c0 = 256u * b + 4u * lane;
     if (a.y) {
-        typename Elem<TYPE>::raw w[4];
+        typename Elem<TYPE>::raw w[V];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = Elem<TYPE>::down((float)(p[j] * root));
-        store_row4<TYPE>(a.y + row * a.dim + c0, n, w);
+        for (uint32_t j = 0; j < V; j++) w[j] = Elem<TYPE>::down((float)(p[j] * root));
+        store_row(a.y + row * a.dim + c0, n, w);
     }
     if (!a.q) return;
-    int32_t sum;
-    const uint32_t packed = codes4(p, factor, sum);
-    if (a.format == PULSAR_ROWS_Q8_K) {
-        uint8_t *ob = a.q + (row * ((a.dim + 255u) / 256u) + b) * 292u;
-        sum = group_sum<4>(sum);
-        __builtin_memcpy(ob + 4u + 4u * lane, &packed, 4);
-        if ((lane & 3u) == 0u) {
-            const int16_t s16 = (int16_t)sum;
-            __builtin_memcpy(ob + 260u + 2u * (lane >> 2), &s16, 2);
-        }
-        if (lane == 0u) {
-            const float d = (float)(__builtin_bit_cast(double, top) * root * (1.0 / 127.0));
-            __builtin_memcpy(ob, &d, 4);
-        }
-    } else {
-        store_codes(a.q + row * a.q_stride + c0, n, packed);
+    int8_t q[V];
+    int32_t sum = codes_of(p, factor, q);
+    if (a.format == PULSAR_ROWS_I8) {
+        store_row((int8_t *)a.q + row * a.q_stride + c0, n, q);
+        return;
+    }
+    sum = group_sum<16u / V>(sum);
+    if (c0 >= ((a.dim + 255u) & ~255u)) return;  // the second block of a chunk may not be there
+    uint8_t *ob = a.q + (row * ((a.dim + 255u) / 256u) + c0 / 256u) * 292u;
+    const uint32_t at = c0 % 256u;
+    __builtin_memcpy(ob + 4u + at, q, V);
+    if (at % 16u == 0u) {
+        const int16_t s16 = (int16_t)sum;
+        __builtin_memcpy(ob + 260u + at / 8u, &s16, 2);
+    }
+    if (at == 0u) {
+        const float d = (float)(__builtin_bit_cast(double, top) * root * (1.0 / 127.0));
+        __builtin_memcpy(ob, &d, 4);
     }
 }
 
-// How many of the 4 values from c0 on are in the row
-PK_DEV uint32_t inside(uint32_t c0, uint32_t dim) { return c0 < dim ? (dim - c0 < 4u ? dim - c0 : 4u) : 0u; }
-
 template <uint32_t TYPE, uint32_t NB>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
+    constexpr uint32_t V = kLane<TYPE>;
+    typedef typename Elem<TYPE>::raw raw;
     __shared__ RowStats lds;
     const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_chunk = (a.dim + 255u) / 256u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t row = blockIdx.x;
-    double p[NB][4], ss = 0.0;
-    uint64_t top[NB];
-    float s[NB][4];
+    const bool blocks = a.format == PULSAR_ROWS_Q8_K;
+    auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
+    double ss = 0.0;
+    uint64_t top[NB], row_top = 0u;
+    // held over the exchange in the rows' type, a quarter of the products' registers: two
+    // blocks of a row of 14336 values fit a CU, and the products cost 5 operations again
+    raw held[NB][V];
+    {
+        float s[NB][V];
 #pragma unroll
-    for (uint32_t j = 0; j < NB; j++) {
-        const uint32_t b = wave + waves * j, c0 = 256u * b + 4u * lane;
-        norm_load<TYPE>(a, a.x + row * a.x_stride + c0, a.residual + row * a.res_stride + c0, inside(c0, a.dim), s[j]);
-    }
+        for (uint32_t j = 0; j < NB; j++) norm_load(a, row, first(j), inside<V>(first(j), a.dim), s[j]);
 #pragma unroll
-    for (uint32_t j = 0; j < NB; j++) {
-        const uint32_t b = wave + waves * j, c0 = 256u * b + 4u * lane, n = inside(c0, a.dim);
-        if (a.sum) norm_put_sum<TYPE>(a.sum + row * a.sum_stride + c0, n, s[j]);
-        float g[4];
-        load_row4<PULSAR_TYPE_F32>(a.gain + c0, n, g);
-        top[j] = 0u;
+        for (uint32_t j = 0; j < NB; j++) {
+            const uint32_t n = inside<V>(first(j), a.dim);
+            double p[V];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const double v = s[j][k];
-            ss = __builtin_fma(v, v, ss);
-            p[j][k] = v * (double)g[k];
-            top[j] = max_bits(top[j], size_bits(p[j][k]));
+            for (uint32_t k = 0; k < V; k++) held[j][k] = Elem<TYPE>::down(s[j][k]);  // exact
+            if (a.sum) store_row(a.sum + row * a.sum_stride + first(j), n, held[j]);
+            top[j] = norm_products(a, first(j), n, s[j], p, ss);
         }
     }
-    uint64_t row_top = 0u;
-    if (a.format == PULSAR_ROWS_Q8_K) {
 #pragma unroll
-        for (uint32_t j = 0; j < NB; j++) top[j] = wave_max64(top[j]);
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < NB; j++) row_top = max_bits(row_top, top[j]);
-        row_top = wave_max64(row_top);
+    for (uint32_t j = 0; j < NB; j++) {
+        if (blocks)
+            top[j] = group_max64<256u / V>(top[j]);
+        else
+            row_top = max_bits(row_top, top[j]);
     }
+    if (!blocks) row_top = group_max64<64>(row_top);
     ss = wave_sum64(ss);
     block_stats(lds, ss, row_top);
     const double root = norm_root(ss, a.dim, a.eps);
     const double row_factor = code_factor(__builtin_bit_cast(double, row_top));
 #pragma unroll
     for (uint32_t j = 0; j < NB; j++) {
-        const uint32_t b = wave + waves * j, c0 = 256u * b + 4u * lane;
-        if (b >= n_chunk) break;  // wave-uniform
-        const bool blocks = a.format == PULSAR_ROWS_Q8_K;
-        norm_put<TYPE>(a, row, b, inside(c0, a.dim), p[j], root, blocks ? top[j] : row_top,
-                       blocks ? code_factor(__builtin_bit_cast(double, top[j])) : row_factor);
+        if (64u * V * (wave + waves * j) >= a.dim) break;  // wave-uniform
+        const uint32_t n = inside<V>(first(j), a.dim);
+        float s[V];
+        double p[V], unused = 0.0;
+#pragma unroll
+        for (uint32_t k = 0; k < V; k++) s[k] = Elem<TYPE>::up(held[j][k]);
+        norm_products(a, first(j), n, s, p, unused);
+        norm_put(a, row, first(j), n, p, root, blocks ? top[j] : row_top,
+                 blocks ? code_factor(__builtin_bit_cast(double, top[j])) : row_factor);
     }
     if (a.scales && threadIdx.x == 0u)
         a.scales[row] = (float)(__builtin_bit_cast(double, row_top) * root * (1.0 / 127.0));
@@ -184,50 +206,36 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
 // is written (x and residual may be gone by then)
 template <uint32_t TYPE>
 __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs<TYPE> a) {
+    constexpr uint32_t V = kLane<TYPE>;
     __shared__ RowStats lds;
-    const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_chunk = (a.dim + 255u) / 256u;
+    const uint32_t step = V * blockDim.x;
     const uint64_t row = blockIdx.x;
-    const typename Elem<TYPE>::raw *x = a.x + row * a.x_stride, *res = a.residual + row * a.res_stride;
-    double ss = 0.0;
+    const bool blocks = a.format == PULSAR_ROWS_Q8_K;
+    double ss = 0.0, p[V];
     uint64_t row_top = 0u;
-    for (uint32_t b = wave; b < n_chunk; b += waves) {
-        const uint32_t c0 = 256u * b + 4u * lane, n = inside(c0, a.dim);
-        float s[4], g[4];
-        norm_load<TYPE>(a, x + c0, res + c0, n, s);
-        if (a.sum) norm_put_sum<TYPE>(a.sum + row * a.sum_stride + c0, n, s);
-        load_row4<PULSAR_TYPE_F32>(a.gain + c0, n, g);
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const double v = s[k];
-            ss = __builtin_fma(v, v, ss);
-            row_top = max_bits(row_top, size_bits(v * (double)g[k]));
-        }
+    float s[V];
+    for (uint32_t c0 = V * threadIdx.x; c0 < a.dim; c0 += step) {
+        const uint32_t n = inside<V>(c0, a.dim);
+        norm_load(a, row, c0, n, s);
+        if (a.sum) norm_put_sum(a, row, c0, n, s);
+        row_top = max_bits(row_top, norm_products(a, c0, n, s, p, ss));
     }
     ss = wave_sum64(ss);
-    row_top = wave_max64(row_top);
+    row_top = group_max64<64>(row_top);
     block_stats(lds, ss, row_top);
     const double root = norm_root(ss, a.dim, a.eps);
     const double row_factor = code_factor(__builtin_bit_cast(double, row_top));
-    for (uint32_t b = wave; b < n_chunk; b += waves) {
-        const uint32_t c0 = 256u * b + 4u * lane, n = inside(c0, a.dim);
-        float s[4], g[4];
+    const uint32_t chunks = (a.dim + 64u * V - 1u) / (64u * V);  // whole waves: lanes exchange
+    for (uint32_t c0 = V * threadIdx.x; c0 / (64u * V) < chunks; c0 += step) {
+        const uint32_t n = inside<V>(c0, a.dim);
         if (a.sum)
-            load_row4<TYPE>(a.sum + row * a.sum_stride + c0, n, s);  // this lane's own stores
+            load_row<TYPE>(a.sum + row * a.sum_stride + c0, n, s);  // this lane's own stores
         else
-            norm_load<TYPE>(a, x + c0, res + c0, n, s);
-        load_row4<PULSAR_TYPE_F32>(a.gain + c0, n, g);
-        double p[4];
-        uint64_t top = 0u;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            p[k] = (double)s[k] * (double)g[k];
-            top = max_bits(top, size_bits(p[k]));
-        }
-        const bool blocks = a.format == PULSAR_ROWS_Q8_K;
-        top = blocks ? wave_max64(top) : row_top;
-        norm_put<TYPE>(a, row, b, n, p, root, top,
-                       blocks ? code_factor(__builtin_bit_cast(double, top)) : row_factor);
+            norm_load(a, row, c0, n, s);
+        double unused = 0.0;
+        uint64_t top = norm_products(a, c0, n, s, p, unused);
+        top = blocks ? group_max64<256u / V>(top) : row_top;
+        norm_put(a, row, c0, n, p, root, top, blocks ? code_factor(__builtin_bit_cast(double, top)) : row_factor);
     }
     if (a.scales && threadIdx.x == 0u)
         a.scales[row] = (float)(__builtin_bit_cast(double, row_top) * root * (1.0 / 127.0));
@@ -277,87 +285,208 @@ struct QuantArgs {
     uint32_t dim, act_op;
 };
 
-template <uint32_t TYPE>
-PK_DEV void quant_values(const QuantArgs<TYPE> &a, const typename Elem<TYPE>::raw *x,
-                         const typename Elem<TYPE>::raw *up, uint32_t n, double (&v)[4]) {
-    float g[4], u[4];
-    load_row4<TYPE>(x, n, g);
+template <uint32_t TYPE, uint32_t V>
+PK_DEV void quant_values(const QuantArgs<TYPE> &a, uint64_t row, uint32_t c0, uint32_t n, double (&v)[V]) {
+    float g[V], u[V];
+    load_row<TYPE>(a.x + row * a.x_stride + c0, n, g);
     if (a.up) {
-        load_row4<TYPE>(up, n, u);
+        load_row<TYPE>(a.up + row * a.up_stride + c0, n, u);
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = glu64(g[k], u[k], a.act_op);
+        for (uint32_t k = 0; k < V; k++) v[k] = glu64(g[k], u[k], a.act_op);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = g[k];
+        for (uint32_t k = 0; k < V; k++) v[k] = g[k];
     }
 }
+// A row of any length and values, read twice and combined in 64 bits
+template <uint32_t TYPE>
+PK_DEV void quantize_row(const QuantArgs<TYPE> &a, RowStats &lds) {
+    constexpr uint32_t V = kLane<TYPE>;
+    const uint32_t step = V * blockDim.x;
+    const uint64_t row = blockIdx.x;
+    double v[V], none = 0.0;
+    uint64_t top = 0u;
+    for (uint32_t c0 = V * threadIdx.x; c0 < a.dim; c0 += step) {
+        quant_values(a, row, c0, inside<V>(c0, a.dim), v);
+#pragma unroll
+        for (uint32_t k = 0; k < V; k++) top = max_bits(top, size_bits(v[k]));
+    }
+    top = group_max64<64>(top);
+    block_stats(lds, none, top);
+    const double largest = __builtin_bit_cast(double, top), factor = code_factor(largest);
+    for (uint32_t c0 = V * threadIdx.x; c0 < a.dim; c0 += step) {
+        const uint32_t n = inside<V>(c0, a.dim);
+        quant_values(a, row, c0, n, v);
+        int8_t q[V];
+        codes_of(v, factor, q);
+        store_row((int8_t *)a.q + row * a.q_stride + c0, n, q);
+    }
+    if (threadIdx.x == 0u) a.scales[row] = (float)(largest * (1.0 / 127.0));
+}
+template <uint32_t TYPE>
+__global__ __launch_bounds__(1024) void quantize_i8_long_kernel(QuantArgs<TYPE> a) {
+    __shared__ RowStats lds;
+    quantize_row(a, lds);
+}
 
+// x as it is
 template <uint32_t TYPE, uint32_t NB>
 __global__ __launch_bounds__(1024) void quantize_i8_kernel(QuantArgs<TYPE> a) {
+    constexpr uint32_t V = kLane<TYPE>;
     __shared__ RowStats lds;
     const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t row = blockIdx.x;
-    double v[NB][4], none = 0.0;
-    uint64_t top = 0u;
+    auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
+    float x[NB][V];
+    double none = 0.0;
+    uint32_t top32 = 0u;
 #pragma unroll
     for (uint32_t j = 0; j < NB; j++) {
-        const uint32_t c0 = 256u * (wave + waves * j) + 4u * lane;
-        quant_values<TYPE>(a, a.x + row * a.x_stride + c0, a.up + row * a.up_stride + c0, inside(c0, a.dim), v[j]);
+        load_row<TYPE>(a.x + row * a.x_stride + first(j), inside<V>(first(j), a.dim), x[j]);
 #pragma unroll
-        for (int k = 0; k < 4; k++) top = max_bits(top, size_bits(v[j][k]));
+        for (uint32_t k = 0; k < V; k++) {
+            const uint32_t w = __float_as_uint(x[j][k]) & 0x7fffffffu;
+            top32 = top32 > w ? top32 : w;
+        }
     }
-    top = wave_max64(top);
+    uint64_t top = group_max64<64>(__builtin_bit_cast(uint64_t, (double)__uint_as_float(top32)));
     block_stats(lds, none, top);
     const double largest = __builtin_bit_cast(double, top), factor = code_factor(largest);
 #pragma unroll
     for (uint32_t j = 0; j < NB; j++) {
-        const uint32_t c0 = 256u * (wave + waves * j) + 4u * lane;
-        int32_t sum;
-        store_codes(a.q + row * a.q_stride + c0, inside(c0, a.dim), codes4(v[j], factor, sum));
+        double v[V];
+        int8_t q[V];
+#pragma unroll
+        for (uint32_t k = 0; k < V; k++) v[k] = x[j][k];
+        codes_of(v, factor, q);
+        store_row((int8_t *)a.q + row * a.q_stride + first(j), inside<V>(first(j), a.dim), q);
     }
     if (threadIdx.x == 0u) a.scales[row] = (float)(largest * (1.0 / 127.0));
 }
 
-// Rows of more values than a block holds: read and combined twice
-template <uint32_t TYPE>
-__global__ __launch_bounds__(1024) void quantize_i8_long_kernel(QuantArgs<TYPE> a) {
-    __shared__ RowStats lds;
-    const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_chunk = (a.dim + 255u) / 256u;
-    const uint64_t row = blockIdx.x;
-    const typename Elem<TYPE>::raw *x = a.x + row * a.x_stride, *up = a.up + row * a.up_stride;
-    double v[4], none = 0.0;
-    uint64_t top = 0u;
-    for (uint32_t b = wave; b < n_chunk; b += waves) {
-        const uint32_t c0 = 256u * b + 4u * lane;
-        quant_values<TYPE>(a, x + c0, up + c0, inside(c0, a.dim), v);
-#pragma unroll
-        for (int k = 0; k < 4; k++) top = max_bits(top, size_bits(v[k]));
+// The gated combine in f32, of relative error below 2^-20: the sigmoid's 4 units and the
+// exponent's part that z's rounding leaves (below 2^-21 together), 5 roundings. Where the
+// gate is below kFar the sigmoid is nearly out of f32's range, and the value is no use.
+constexpr float kFar = -85.0f;
+PK_DEV float glu32(float g, float u, uint32_t op, bool &far) {
+    if (op == PULSAR_ACT_SWIGLU_OAI) {
+        constexpr float kHi = 1.702f, kLo = (float)(1.702 - (double)1.702f);
+        g = g > 7.0f ? 7.0f : g;  // NaN stays
+        u = (u > 7.0f ? 7.0f : u < -7.0f ? -7.0f : u) + 1.0f;
+        const float z = kHi * g, lo = __builtin_fmaf(kLo, g, __builtin_fmaf(kHi, g, -z));
+        const float e = exp_near(-z);
+        far = !(z >= kFar);
+        return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, -lo, e)) * u;
     }
-    top = wave_max64(top);
+    far = !(g >= kFar);
+    return g * sigmoid_near(g) * u;
+}
+
+// glu(x, up): 64 bits decide the codes, but few of them need 64 bits. Of the f32 values,
+// off by 2^-20, those that may be the row's largest are combined again in 64 bits, and
+// those whose code argument (up to 127: off by 2^-13) lies within 2^-12 of a half, one in
+// 2000; a wave with none of either skips it. 30 operations a value in place of 60: 4096
+// rows of 14336 bf16 values 167 -> 139 us (2100 GB/s), 8192 of 4096 65 -> 53 (3200). What
+// is left there is the chain of a row: load, largest, again, codes, with two barriers, and
+// one row of 14 waves on a CU. Holding the next row's values meanwhile, or this one's for
+// the second combine, takes registers that more waves want: 162 and more.
+template <uint32_t TYPE, uint32_t NB>
+__global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
+    constexpr uint32_t V = kLane<TYPE>;
+    typedef typename Elem<TYPE>::raw raw;
+    __shared__ RowStats lds, lds64;
+    const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t row = blockIdx.x;
+    auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
+    const raw *x = a.x + row * a.x_stride, *up = a.up + row * a.up_stride;
+    // value i of the lane (of chunk i / V) in 64 bits
+    auto again = [&](uint32_t i, uint32_t &c) {
+        c = V * (64u * (wave + waves * (i / V)) + lane) + i % V;
+        return glu64(Elem<TYPE>::up(x[c]), Elem<TYPE>::up(up[c]), a.act_op);
+    };
+    float v[NB][V];
+    uint32_t far = 0u, top32 = 0u;  // far: a bit a value
+#pragma unroll
+    for (uint32_t j = 0; j < NB; j++) {
+        float g[V], u[V];
+        const uint32_t n = inside<V>(first(j), a.dim);
+        load_row<TYPE>(x + first(j), n, g);
+        load_row<TYPE>(up + first(j), n, u);
+#pragma unroll
+        for (uint32_t k = 0; k < V; k++) {
+            bool f;
+            v[j][k] = glu32(g[k], u[k], a.act_op, f);
+            if (f) far |= 1u << (j * V + k);  // not behind the row's end: 0 there
+            const uint32_t w = __float_as_uint(v[j][k]) & 0x7fffffffu;
+            top32 = top32 > w ? top32 : w;
+        }
+    }
+    double none = 0.0;
+    uint64_t top = group_max64<64>(top32);
     block_stats(lds, none, top);
+    // zeros, values at the ends of f32's range, infinity, NaN
+    const float about = __uint_as_float((uint32_t)top);
+    if (!(about >= 1e-30f && about <= 1e30f)) {  // block-uniform
+        __syncthreads();
+        quantize_row(a, lds);
+        return;
+    }
+    uint32_t todo = far;
+    const float least = about * (1.0f - 0x1p-18f);
+#pragma unroll
+    for (uint32_t j = 0; j < NB; j++)
+#pragma unroll
+        for (uint32_t k = 0; k < V; k++)
+            if (__builtin_fabsf(v[j][k]) >= least) todo |= 1u << (j * V + k);
+    top = 0u;
+    uint32_t c;
+    for (; todo; todo &= todo - 1u) top = max_bits(top, size_bits(again(__builtin_ctz(todo), c)));
+    top = group_max64<64>(top);
+    block_stats(lds64, none, top);
     const double largest = __builtin_bit_cast(double, top), factor = code_factor(largest);
-    for (uint32_t b = wave; b < n_chunk; b += waves) {
-        const uint32_t c0 = 256u * b + 4u * lane, n = inside(c0, a.dim);
-        quant_values<TYPE>(a, x + c0, up + c0, n, v);
-        int32_t sum;
-        store_codes(a.q + row * a.q_stride + c0, n, codes4(v, factor, sum));
+    const float factor32 = (float)factor;
+    todo = far;
+#pragma unroll
+    for (uint32_t j = 0; j < NB; j++) {
+        int8_t q[V];
+#pragma unroll
+        for (uint32_t k = 0; k < V; k++) {
+            const float t = v[j][k] * factor32, up_by = t + __builtin_copysignf(0.5f, t);
+            q[k] = (int8_t)(int32_t)up_by;
+            // t within 2^-12 of a half: up_by of a whole number
+            if (__builtin_fabsf(up_by - __builtin_rintf(up_by)) < 0x1p-12f) todo |= 1u << (j * V + k);
+        }
+        store_row((int8_t *)a.q + row * a.q_stride + first(j), inside<V>(first(j), a.dim), q);
+    }
+    for (; todo; todo &= todo - 1u) {
+        const double w = again(__builtin_ctz(todo), c);
+        if (c < a.dim) *(volatile PK_GLOBAL int8_t *)(a.q + row * a.q_stride + c) = (int8_t)code_of(w, factor);
     }
     if (threadIdx.x == 0u) a.scales[row] = (float)(largest * (1.0 / 127.0));
 }
 
 // ---------------------------------------------------------------- launch --
 
-// Waves and chunks of a wave for rows of n_chunk chunks; 0: the row is too long
+// Waves and chunks of a wave for rows of n_chunk chunks; 0 chunks: more than a block holds
 struct RowShape {
     uint32_t waves, chunks;
 };
-static RowShape row_shape(uint32_t n_chunk) {
-    for (uint32_t nb = 1; nb <= 4u; nb <<= 1)
+// Few rows take as many waves as there are chunks (norm of one row of 4096 bf16 values
+// 4.3 us, with two chunks a wave 4.7). Many rows want fewer waves to start and more of a
+// row on its way in each: two chunks (8192 rows of 4096 bf16 values, combined: 53 us, one
+// chunk 68), four of f32 rows that would take more than 8 waves else (norm of 4096 rows of
+// 8192: 114 against 132).
+static RowShape row_shape(uint32_t n_chunk, uint32_t n_rows, uint32_t most) {
+    uint32_t nb = n_rows < 256u || n_chunk == 1u ? 1u : n_chunk > 16u && most > 2u ? 4u : 2u;
+    for (; nb <= most; nb <<= 1)
         if (n_chunk <= 16u * nb) return {(n_chunk + nb - 1u) / nb, nb};
     return {16u, 0u};
 }
+// 16384 values in a block of 16 waves
+template <uint32_t TYPE>
+constexpr uint32_t kMostChunks = 16u / kLane<TYPE>;
 
 // Rows that may be written while those of `in` are read: the same rows
 static bool same_rows(const void *out, uint64_t out_stride, const void *in, uint64_t in_stride) {
@@ -372,14 +501,16 @@ static int launch_norm(void *q, void *scales, void *y, void *sum, const void *x,
     const NormArgs<TYPE> a = {(uint8_t *)q, (float *)scales, (raw *)y, (raw *)sum, (const raw *)x,
                               (const raw *)residual, (const float *)gain, x_stride, res_stride, sum_stride, q_stride,
                               dim, format, eps};
-    const RowShape s = row_shape((dim + 255u) / 256u);
+    const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kMostChunks<TYPE>);
     const dim3 grid(n_rows), block(64u * s.waves);
-    switch (s.chunks) {
-    case 1: hipLaunchKernelGGL((norm_kernel<TYPE, 1>), grid, block, 0, pk::stream(), a); break;
-    case 2: hipLaunchKernelGGL((norm_kernel<TYPE, 2>), grid, block, 0, pk::stream(), a); break;
-    case 4: hipLaunchKernelGGL((norm_kernel<TYPE, 4>), grid, block, 0, pk::stream(), a); break;
-    default: hipLaunchKernelGGL((norm_long_kernel<TYPE>), grid, block, 0, pk::stream(), a);
-    }
+    if (s.chunks == 1u)
+        hipLaunchKernelGGL((norm_kernel<TYPE, 1>), grid, block, 0, pk::stream(), a);
+    else if (s.chunks == 2u)
+        hipLaunchKernelGGL((norm_kernel<TYPE, 2>), grid, block, 0, pk::stream(), a);
+    else if (s.chunks != 0u)
+        hipLaunchKernelGGL((norm_kernel<TYPE, kMostChunks<TYPE>>), grid, block, 0, pk::stream(), a);
+    else
+        hipLaunchKernelGGL((norm_long_kernel<TYPE>), grid, block, 0, pk::stream(), a);
     return launch_ok("rms_norm_q8 launch");
 }
 
@@ -389,14 +520,24 @@ static int launch_quantize(void *q, void *scales, const void *x, const void *up,
     typedef typename Elem<TYPE>::raw raw;
     const QuantArgs<TYPE> a = {(uint8_t *)q, (float *)scales, (const raw *)x, (const raw *)up, x_stride, up_stride,
                                q_stride, dim, act_op};
-    const RowShape s = row_shape((dim + 255u) / 256u);
+    const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kMostChunks<TYPE>);
     const dim3 grid(n_rows), block(64u * s.waves);
-    switch (s.chunks) {
-    case 1: hipLaunchKernelGGL((quantize_i8_kernel<TYPE, 1>), grid, block, 0, pk::stream(), a); break;
-    case 2: hipLaunchKernelGGL((quantize_i8_kernel<TYPE, 2>), grid, block, 0, pk::stream(), a); break;
-    case 4: hipLaunchKernelGGL((quantize_i8_kernel<TYPE, 4>), grid, block, 0, pk::stream(), a); break;
-    default: hipLaunchKernelGGL((quantize_i8_long_kernel<TYPE>), grid, block, 0, pk::stream(), a);
-    }
+#define PK_QUANT_NB(NB)                                                                        \
+    do {                                                                                       \
+        if (up)                                                                                \
+            hipLaunchKernelGGL((glu_i8_kernel<TYPE, NB>), grid, block, 0, pk::stream(), a);      \
+        else                                                                                   \
+            hipLaunchKernelGGL((quantize_i8_kernel<TYPE, NB>), grid, block, 0, pk::stream(), a); \
+    } while (0)
+    if (s.chunks == 1u)
+        PK_QUANT_NB(1);
+    else if (s.chunks == 2u)
+        PK_QUANT_NB(2);
+    else if (s.chunks != 0u)
+        PK_QUANT_NB(kMostChunks<TYPE>);
+    else
+        hipLaunchKernelGGL((quantize_i8_long_kernel<TYPE>), grid, block, 0, pk::stream(), a);
+#undef PK_QUANT_NB
     return launch_ok("quantize_i8 launch");
 }
 
