@@ -141,8 +141,8 @@ int pulsar_matmul_kq(void *out, const void *w, const void *xq, uint32_t in_dim,
  * from 0, decided as it stands in 64 bits (an argument nearer than 2^-40 to a half
  * counts as on it); the scale is A / 127, rounded to f32. A row of zeros has codes and
  * scale 0. Where a row (block) holds a NaN its scale is NaN, where it holds an infinity
- * the scale is infinite (in the norm, whose root is infinite then, NaN); the codes of
- * what is not finite are 0. Strides count elements (bytes in int8 rows), 0 stands for
+ * the scale is infinite (in the norm, where a row's infinity makes the root 0, NaN; one
+ * of the two where a gain is not finite); the codes of what is not finite are 0. Strides count elements (bytes in int8 rows), 0 stands for
  * packed rows; what lies between rows is left as it is. */
 
 /* s = x + residual (NULL: x), rounded to `type`; y = s * gain / sqrt(mean(s^2) + eps)

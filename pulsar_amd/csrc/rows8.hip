@@ -9,8 +9,8 @@
 // gain, known without it. Sums, products and codes in 64 bits cost about what the bytes
 // do: a value is 5 to 17 bytes of traffic and some 20 operations, most of them at the rate
 // of f32's. Measured (GB/s of what has to move): norm of 8192 rows of 4096 bf16 values to
-// int8 55 us (4270), to q8_K with y 69 (4440), of 2048 rows of f32 32 (4490), quantized as
-// they are 19 (5300).
+// int8 59 us (3970), to q8_K with y 70 (4390), of 2048 rows of f32 32 (4490), quantized as
+// they are 21 (4750), combined by glu first 52 (3250; see there).
 #include "pk_elem.h"
 #include "pk_epilogue.h"
 
@@ -76,7 +76,7 @@ struct NormArgs {
     float eps;
 };
 
-// s of V values: x + residual, rounded to the rows' type
+// s of V values: x + residual, rounded to the rows' type. n: constant where a chunk is whole
 template <uint32_t TYPE, uint32_t V>
 PK_DEV void norm_load(const NormArgs<TYPE> &a, uint64_t row, uint32_t c0, uint32_t n, float (&s)[V]) {
     load_row<TYPE>(a.x + row * a.x_stride + c0, n, s);
@@ -93,21 +93,22 @@ PK_DEV void norm_put_sum(const NormArgs<TYPE> &a, uint64_t row, uint32_t c0, uin
     for (uint32_t j = 0; j < V; j++) w[j] = Elem<TYPE>::down(s[j]);  // exact
     store_row(a.sum + row * a.sum_stride + c0, n, w);
 }
-// p = s * gain (exact), the squares of s added to ss, the largest |p|
+// p = s * gain (exact), the squares of s added to ss, the largest |p|, as bits
 template <uint32_t TYPE, uint32_t V>
 PK_DEV uint64_t norm_products(const NormArgs<TYPE> &a, uint32_t c0, uint32_t n, const float (&s)[V], double (&p)[V],
                               double &ss) {
     float g[V];
     load_row<PULSAR_TYPE_F32>(a.gain + c0, n, g);
-    uint64_t top = 0u;
+    double top = 0.0, poison = 0.0;  // a maximum passes over a NaN
 #pragma unroll
     for (uint32_t j = 0; j < V; j++) {
         const double v = s[j];
         ss = __builtin_fma(v, v, ss);
         p[j] = v * (double)g[j];
-        top = max_bits(top, size_bits(p[j]));
+        top = __builtin_fmax(top, __builtin_fabs(p[j]));
+        poison = __builtin_fma(p[j], 0.0, poison);
     }
-    return top;
+    return size_bits(poison != poison && top < __builtin_inf() ? poison : top);
 }
 PK_DEV double norm_root(double sum, uint32_t dim, float eps) {
     const double m = sum / (double)dim + (double)eps;
@@ -190,11 +191,11 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
     for (uint32_t j = 0; j < NB; j++) {
         if (64u * V * (wave + waves * j) >= a.dim) break;  // wave-uniform
         const uint32_t n = inside<V>(first(j), a.dim);
-        float s[V];
-        double p[V], unused = 0.0;
+        float g[V];
+        double p[V];
+        load_row<PULSAR_TYPE_F32>(a.gain + first(j), n, g);
 #pragma unroll
-        for (uint32_t k = 0; k < V; k++) s[k] = Elem<TYPE>::up(held[j][k]);
-        norm_products(a, first(j), n, s, p, unused);
+        for (uint32_t k = 0; k < V; k++) p[k] = (double)Elem<TYPE>::up(held[j][k]) * (double)g[k];
         norm_put(a, row, first(j), n, p, root, blocks ? top[j] : row_top,
                  blocks ? code_factor(__builtin_bit_cast(double, top[j])) : row_factor);
     }
@@ -367,30 +368,33 @@ __global__ __launch_bounds__(1024) void quantize_i8_kernel(QuantArgs<TYPE> a) {
 
 // The gated combine in f32, of relative error below 2^-20: the sigmoid's 4 units and the
 // exponent's part that z's rounding leaves (below 2^-21 together), 5 roundings. Where the
-// gate is below kFar the sigmoid is nearly out of f32's range, and the value is no use.
+// sigmoid's argument z is below kFar it is nearly out of f32's range, and the value no use.
 constexpr float kFar = -85.0f;
-PK_DEV float glu32(float g, float u, uint32_t op, bool &far) {
+PK_DEV float glu32(float g, float u, uint32_t op, float &z) {
     if (op == PULSAR_ACT_SWIGLU_OAI) {
         constexpr float kHi = 1.702f, kLo = (float)(1.702 - (double)1.702f);
         g = g > 7.0f ? 7.0f : g;  // NaN stays
         u = (u > 7.0f ? 7.0f : u < -7.0f ? -7.0f : u) + 1.0f;
-        const float z = kHi * g, lo = __builtin_fmaf(kLo, g, __builtin_fmaf(kHi, g, -z));
-        const float e = exp_near(-z);
-        far = !(z >= kFar);
+        z = kHi * g;
+        const float lo = __builtin_fmaf(kLo, g, __builtin_fmaf(kHi, g, -z)), e = exp_near(-z);
         return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, -lo, e)) * u;
     }
-    far = !(g >= kFar);
+    z = g;
     return g * sigmoid_near(g) * u;
 }
+// What passes NaN on: one instruction for three values
+PK_DEV float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
+PK_DEV float min3(float a, float b, float c) { return __builtin_elementwise_minimum(__builtin_elementwise_minimum(a, b), c); }
 
 // glu(x, up): 64 bits decide the codes, but few of them need 64 bits. Of the f32 values,
 // off by 2^-20, those that may be the row's largest are combined again in 64 bits, and
 // those whose code argument (up to 127: off by 2^-13) lies within 2^-12 of a half, one in
-// 2000; a wave with none of either skips it. 30 operations a value in place of 60: 4096
-// rows of 14336 bf16 values 167 -> 139 us (2100 GB/s), 8192 of 4096 65 -> 53 (3200). What
-// is left there is the chain of a row: load, largest, again, codes, with two barriers, and
-// one row of 14 waves on a CU. Holding the next row's values meanwhile, or this one's for
-// the second combine, takes registers that more waves want: 162 and more.
+// 2000. The common way only asks a lane's largest and its nearest to a half; a lane with
+// some looks for which. Bound by its instructions, two transcendental ones among them: of
+// 8192 rows of 4096 bf16 values the pipes are busy all of 52 us (59 with a mask kept for
+// every value). 14 waves a row of 14336 leave one row to a CU, whose exchanges nothing
+// covers: 4096 rows 111 us, 2640 GB/s (140, and 175 with every value combined in 64 bits);
+// with registers for two rows a CU the compiler spills, and it takes 128.
 template <uint32_t TYPE, uint32_t NB>
 __global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
     constexpr uint32_t V = kLane<TYPE>;
@@ -400,31 +404,34 @@ __global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t row = blockIdx.x;
     auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
+    auto whole = [&](uint32_t j) { return 64u * V * (wave + waves * j + 1u) <= a.dim; };  // wave-uniform
     const raw *x = a.x + row * a.x_stride, *up = a.up + row * a.up_stride;
     // value i of the lane (of chunk i / V) in 64 bits
     auto again = [&](uint32_t i, uint32_t &c) {
         c = V * (64u * (wave + waves * (i / V)) + lane) + i % V;
         return glu64(Elem<TYPE>::up(x[c]), Elem<TYPE>::up(up[c]), a.act_op);
     };
-    float v[NB][V];
-    uint32_t far = 0u, top32 = 0u;  // far: a bit a value
+    float v[NB][V], most = 0.0f, lowest = 0.0f;  // the lane's largest, and its least z
 #pragma unroll
     for (uint32_t j = 0; j < NB; j++) {
-        float g[V], u[V];
-        const uint32_t n = inside<V>(first(j), a.dim);
-        load_row<TYPE>(x + first(j), n, g);
-        load_row<TYPE>(up + first(j), n, u);
+        float g[V], u[V], z[V];
+        if (whole(j)) {
+            load_row<TYPE>(x + first(j), V, g);
+            load_row<TYPE>(up + first(j), V, u);
+        } else {
+            load_row<TYPE>(x + first(j), inside<V>(first(j), a.dim), g);
+            load_row<TYPE>(up + first(j), inside<V>(first(j), a.dim), u);
+        }
 #pragma unroll
-        for (uint32_t k = 0; k < V; k++) {
-            bool f;
-            v[j][k] = glu32(g[k], u[k], a.act_op, f);
-            if (f) far |= 1u << (j * V + k);  // not behind the row's end: 0 there
-            const uint32_t w = __float_as_uint(v[j][k]) & 0x7fffffffu;
-            top32 = top32 > w ? top32 : w;
+        for (uint32_t k = 0; k < V; k++) v[j][k] = glu32(g[k], u[k], a.act_op, z[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < V; k += 2u) {
+            most = max3(most, __builtin_fabsf(v[j][k]), __builtin_fabsf(v[j][k + 1u]));
+            lowest = min3(lowest, z[k], z[k + 1u]);
         }
     }
     double none = 0.0;
-    uint64_t top = group_max64<64>(top32);
+    uint64_t top = group_max64<64>(__float_as_uint(most) & 0x7fffffffu);
     block_stats(lds, none, top);
     // zeros, values at the ends of f32's range, infinity, NaN
     const float about = __uint_as_float((uint32_t)top);
@@ -433,13 +440,18 @@ __global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
         quantize_row(a, lds);
         return;
     }
+    uint32_t far = 0u;  // a bit a value: all of a lane's in the row, where one is far
+    if (!(lowest >= kFar)) {
+#pragma unroll
+        for (uint32_t j = 0; j < NB; j++) far |= ((1u << inside<V>(first(j), a.dim)) - 1u) << (j * V);
+    }
     uint32_t todo = far;
     const float least = about * (1.0f - 0x1p-18f);
+    if (most >= least) {
 #pragma unroll
-    for (uint32_t j = 0; j < NB; j++)
-#pragma unroll
-        for (uint32_t k = 0; k < V; k++)
-            if (__builtin_fabsf(v[j][k]) >= least) todo |= 1u << (j * V + k);
+        for (uint32_t i = 0; i < NB * V; i++)
+            if (__builtin_fabsf(v[i / V][i % V]) >= least) todo |= 1u << i;
+    }
     top = 0u;
     uint32_t c;
     for (; todo; todo &= todo - 1u) top = max_bits(top, size_bits(again(__builtin_ctz(todo), c)));
@@ -447,22 +459,38 @@ __global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
     block_stats(lds64, none, top);
     const double largest = __builtin_bit_cast(double, top), factor = code_factor(largest);
     const float factor32 = (float)factor;
-    todo = far;
+    // code + 128 as an unsigned byte, rounded by the conversion
+    auto argument = [&](uint32_t i) { return __builtin_fmaf(v[i / V][i % V], factor32, 128.0f); };
+    auto off_half = [&](uint32_t i) { return __builtin_amdgcn_fractf(argument(i)) - 0.5f; };
+    float nearest = 1.0f;
 #pragma unroll
     for (uint32_t j = 0; j < NB; j++) {
+        uint32_t words[V / 4u] = {};
         int8_t q[V];
 #pragma unroll
-        for (uint32_t k = 0; k < V; k++) {
-            const float t = v[j][k] * factor32, up_by = t + __builtin_copysignf(0.5f, t);
-            q[k] = (int8_t)(int32_t)up_by;
-            // t within 2^-12 of a half: up_by of a whole number
-            if (__builtin_fabsf(up_by - __builtin_rintf(up_by)) < 0x1p-12f) todo |= 1u << (j * V + k);
-        }
-        store_row((int8_t *)a.q + row * a.q_stride + first(j), inside<V>(first(j), a.dim), q);
+        for (uint32_t k = 0; k < V; k++)
+            words[k / 4u] = __builtin_amdgcn_cvt_pk_u8_f32(argument(j * V + k), k % 4u, words[k / 4u]);
+#pragma unroll
+        for (uint32_t k = 0; k < V; k += 2u)
+            nearest = min3(nearest, __builtin_fabsf(off_half(j * V + k)), __builtin_fabsf(off_half(j * V + k + 1u)));
+#pragma unroll
+        for (uint32_t k = 0; k < V / 4u; k++) words[k] ^= 0x80808080u;
+        __builtin_memcpy(q, words, V);
+        int8_t *to = (int8_t *)a.q + row * a.q_stride + first(j);
+        if (whole(j))
+            store_row(to, V, q);
+        else
+            store_row(to, inside<V>(first(j), a.dim), q);
+    }
+    todo = far;
+    if (nearest < 0x1p-12f) {
+#pragma unroll
+        for (uint32_t i = 0; i < NB * V; i++)
+            if (__builtin_fabsf(off_half(i)) < 0x1p-12f) todo |= 1u << i;
     }
     for (; todo; todo &= todo - 1u) {
         const double w = again(__builtin_ctz(todo), c);
-        if (c < a.dim) *(volatile PK_GLOBAL int8_t *)(a.q + row * a.q_stride + c) = (int8_t)code_of(w, factor);
+        *(volatile PK_GLOBAL int8_t *)(a.q + row * a.q_stride + c) = (int8_t)code_of(w, factor);
     }
     if (threadIdx.x == 0u) a.scales[row] = (float)(largest * (1.0 / 127.0));
 }
