@@ -366,9 +366,11 @@ __global__ __launch_bounds__(1024) void quantize_i8_kernel(QuantArgs<TYPE> a) {
     if (threadIdx.x == 0u) a.scales[row] = (float)(largest * (1.0 / 127.0));
 }
 
-// The gated combine in f32, of relative error below 2^-20: the sigmoid's 4 units and the
-// exponent's part that z's rounding leaves (below 2^-21 together), 5 roundings. Where the
-// sigmoid's argument z is below kFar it is nearly out of f32's range, and the value no use.
+// The gated combine in f32, of relative error below 2^-20 (or a step of f32's least
+// numbers): the sigmoid's 4 units and the exponent's part that z's rounding leaves (below
+// 2^-21 together), 5 roundings. Where the sigmoid's argument z is below kFar it is nearly
+// out of f32's range, and the value no use. g u comes first: g of f32's least numbers
+// would lose its bits to the sigmoid, and a large u would bring the loss up.
 constexpr float kFar = -85.0f;
 PK_DEV float glu32(float g, float u, uint32_t op, float &z) {
     if (op == PULSAR_ACT_SWIGLU_OAI) {
@@ -380,7 +382,7 @@ PK_DEV float glu32(float g, float u, uint32_t op, float &z) {
         return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, -lo, e)) * u;
     }
     z = g;
-    return g * sigmoid_near(g) * u;
+    return g * u * sigmoid_near(g);
 }
 // What passes NaN on: one instruction for three values
 PK_DEV float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }

@@ -393,3 +393,43 @@ def test_feeds_the_products(dev):
     x = down(a[0]).reshape(3, -1)
     want, scale = oracle.rows_dot(w, rb, 65, x, 768, 3, fm.QUANT_Q4_K, 8)
     assert_rows_close(down(out), want.reshape(3, 65), scale.reshape(3, 65), "dots")
+
+
+@pytest.mark.parametrize("kind", [TYPE_F32, TYPE_BF16], ids=NAMES.get)
+@pytest.mark.parametrize("dim", [300, 5000])
+def test_quantize_least_gates(dev, dim, kind):
+    """Gates at the lowest end of the type, below its normal values too, under values of
+    up that bring the products back to the middle of the range."""
+    rng = np.random.default_rng(dim + kind)
+    e = np.arange(dim) % 25
+    g = rounded(np.ldexp(1 + rng.random((3, dim)), -122 - e), kind)
+    u = rounded(np.ldexp(rng.standard_normal((3, dim)), 100 + e), kind)
+    assert ((g > 0) & (g < 2.0**-126)).any() and np.isfinite(u).all()
+    q, sc = torch.full((3, dim), 99, dtype=torch.int8, device=dev), up_f32(np.full(3, 9))
+    K.quantize_i8(q, sc, dev_rows(g, kind), dev_rows(u, kind), dim, 3, ACT_SILU, kind)
+    quant_check(glu64(g, u, ACT_SILU), q, sc, (dim, NAMES[kind]))
+
+
+@pytest.mark.parametrize("dim", [300, 4096])
+def test_norm_blocks_and_the_f32_quantizer(dev, dim):
+    """The norm's q8_K rows against pulsar_quantize_q8_K of its y: a code differs only
+    where y's rounding and the f32 decision (2^-24 of an argument of up to 127 for y, its
+    block's largest, 1 / d and the product each: 2^-15 together) reach a half, and by 1."""
+    rows = 64
+    n = Norm(rows, dim, TYPE_F32)
+    a = n.arrays(ROWS_Q8_K)
+    n.call(a, ROWS_Q8_K)
+    other = torch.zeros_like(a[0])
+    K.quantize_q8_k(other, a[2], dim, rows)
+    d, codes, _ = split_blocks(a[0], rows, dim)
+    d2, codes2, _ = split_blocks(other, rows, dim)
+    near(d2, d, 4 * 2.0**-24, 0.0, "d")
+    _, p, _ = n.want()
+    nb = -(-dim // 256)
+    blocks = np.zeros((rows, 256 * nb))
+    blocks[:, :dim] = p
+    blocks = blocks.reshape(rows, nb, 256)
+    t = np.abs(blocks) / np.abs(blocks).max(2, keepdims=True) * 127
+    border = np.abs(t - np.floor(t) - 0.5) <= 2.0**-15
+    differ = codes != codes2
+    assert (np.abs(codes - codes2) <= 1).all() and not (differ & ~border).any(), int(differ.sum())
