@@ -3,14 +3,14 @@
 // (pulsar_quantize_i8).
 //
 // A row is one block's: a lane holds 16 bytes of a chunk (a q8_K block of f32 values, two
-// of 16-bit ones), a wave up to four chunks, so that the row is read once, stays in
+// of 16-bit ones), a wave up to eight chunks, so that the row is read once, stays in
 // registers and is written once. The norm needs one exchange between the waves: its root
 // divides every value of the row alike, so codes and the largest size are those of s *
 // gain, known without it. Sums, products and codes in 64 bits cost about what the bytes
 // do: a value is 5 to 17 bytes of traffic and some 20 operations, most of them at the rate
 // of f32's. Measured (GB/s of what has to move): norm of 8192 rows of 4096 bf16 values to
 // int8 59 us (3970), to q8_K with y 70 (4390), of 2048 rows of f32 32 (4490), quantized as
-// they are 21 (4750), combined by glu first 52 (3250; see there).
+// they are 20 (5000), combined by glu first 43 (3900).
 #include "pk_elem.h"
 #include "pk_epilogue.h"
 
@@ -393,10 +393,9 @@ PK_DEV float min3(float a, float b, float c) { return __builtin_elementwise_mini
 // those whose code argument (up to 127: off by 2^-13) lies within 2^-12 of a half, one in
 // 2000. The common way only asks a lane's largest and its nearest to a half; a lane with
 // some looks for which. Bound by its instructions, two transcendental ones among them: of
-// 8192 rows of 4096 bf16 values the pipes are busy all of 52 us (59 with a mask kept for
-// every value). 14 waves a row of 14336 leave one row to a CU, whose exchanges nothing
-// covers: 4096 rows 111 us, 2640 GB/s (140, and 175 with every value combined in 64 bits);
-// with registers for two rows a CU the compiler spills, and it takes 128.
+// 8192 rows of 4096 bf16 values the pipes are busy most of 43 us (59 with a mask kept for
+// every value), 3900 GB/s; 4096 rows of 14336 84 us, 3490 GB/s (175 with every value
+// combined in 64 bits).
 template <uint32_t TYPE, uint32_t NB>
 __global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
     constexpr uint32_t V = kLane<TYPE>;
@@ -505,18 +504,24 @@ struct RowShape {
 };
 // Few rows take as many waves as there are chunks (norm of one row of 4096 bf16 values
 // 4.3 us, with two chunks a wave 4.7). Many rows want fewer waves to start and more of a
-// row on its way in each: two chunks (8192 rows of 4096 bf16 values, combined: 53 us, one
-// chunk 68), four of f32 rows that would take more than 8 waves else (norm of 4096 rows of
-// 8192: 114 against 132).
+// row on its way in each: two chunks (8192 rows of 4096 bf16 values, combined: 43 us, one
+// chunk 60), and twice as many where a row would take more than 12 waves, so that a CU
+// has room for a second (4096 rows of 14336 bf16 values combined 84 against 113, norm of
+// 4096 rows of 8192 f32 values 114 against 133; at 11 waves 81 against 79).
 static RowShape row_shape(uint32_t n_chunk, uint32_t n_rows, uint32_t most) {
-    uint32_t nb = n_rows < 256u || n_chunk == 1u ? 1u : n_chunk > 16u && most > 2u ? 4u : 2u;
-    for (; nb <= most; nb <<= 1)
-        if (n_chunk <= 16u * nb) return {(n_chunk + nb - 1u) / nb, nb};
-    return {16u, 0u};
+    uint32_t nb = 1u;
+    const bool few = n_rows < 256u || n_chunk == 1u;
+    if (!few) nb = 2u;
+    while (nb < most && n_chunk > (few ? 16u : 12u) * nb) nb <<= 1;
+    if (n_chunk > 16u * nb) return {16u, 0u};
+    return {(n_chunk + nb - 1u) / nb, nb};
 }
-// 16384 values in a block of 16 waves
+// Chunks of a wave at most: 16 values a lane in a norm, whose products are of 64 bits
+// (with 32, 2048 rows of 14336 f32 values take 151 us against 133), 32 in the quantizers
 template <uint32_t TYPE>
-constexpr uint32_t kMostChunks = 16u / kLane<TYPE>;
+constexpr uint32_t kNormChunks = 16u / kLane<TYPE>;
+template <uint32_t TYPE>
+constexpr uint32_t kQuantChunks = 32u / kLane<TYPE>;
 
 // Rows that may be written while those of `in` are read: the same rows
 static bool same_rows(const void *out, uint64_t out_stride, const void *in, uint64_t in_stride) {
@@ -531,14 +536,14 @@ static int launch_norm(void *q, void *scales, void *y, void *sum, const void *x,
     const NormArgs<TYPE> a = {(uint8_t *)q, (float *)scales, (raw *)y, (raw *)sum, (const raw *)x,
                               (const raw *)residual, (const float *)gain, x_stride, res_stride, sum_stride, q_stride,
                               dim, format, eps};
-    const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kMostChunks<TYPE>);
+    const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kNormChunks<TYPE>);
     const dim3 grid(n_rows), block(64u * s.waves);
     if (s.chunks == 1u)
         hipLaunchKernelGGL((norm_kernel<TYPE, 1>), grid, block, 0, pk::stream(), a);
     else if (s.chunks == 2u)
         hipLaunchKernelGGL((norm_kernel<TYPE, 2>), grid, block, 0, pk::stream(), a);
     else if (s.chunks != 0u)
-        hipLaunchKernelGGL((norm_kernel<TYPE, kMostChunks<TYPE>>), grid, block, 0, pk::stream(), a);
+        hipLaunchKernelGGL((norm_kernel<TYPE, kNormChunks<TYPE>>), grid, block, 0, pk::stream(), a);
     else
         hipLaunchKernelGGL((norm_long_kernel<TYPE>), grid, block, 0, pk::stream(), a);
     return launch_ok("rms_norm_q8 launch");
@@ -550,7 +555,7 @@ static int launch_quantize(void *q, void *scales, const void *x, const void *up,
     typedef typename Elem<TYPE>::raw raw;
     const QuantArgs<TYPE> a = {(uint8_t *)q, (float *)scales, (const raw *)x, (const raw *)up, x_stride, up_stride,
                                q_stride, dim, act_op};
-    const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kMostChunks<TYPE>);
+    const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kQuantChunks<TYPE>);
     const dim3 grid(n_rows), block(64u * s.waves);
 #define PK_QUANT_NB(NB)                                                                        \
     do {                                                                                       \
@@ -563,8 +568,10 @@ static int launch_quantize(void *q, void *scales, const void *x, const void *up,
         PK_QUANT_NB(1);
     else if (s.chunks == 2u)
         PK_QUANT_NB(2);
+    else if (s.chunks == 4u)
+        PK_QUANT_NB(4);
     else if (s.chunks != 0u)
-        PK_QUANT_NB(kMostChunks<TYPE>);
+        PK_QUANT_NB(kQuantChunks<TYPE>);
     else
         hipLaunchKernelGGL((quantize_i8_long_kernel<TYPE>), grid, block, 0, pk::stream(), a);
 #undef PK_QUANT_NB

@@ -433,3 +433,27 @@ def test_norm_blocks_and_the_f32_quantizer(dev, dim):
     border = np.abs(t - np.floor(t) - 0.5) <= 2.0**-15
     differ = codes != codes2
     assert (np.abs(codes - codes2) <= 1).all() and not (differ & ~border).any(), int(differ.sum())
+
+
+# what a quantizer's block holds and the next; many rows, of as many waves as one row
+# leaves to a second on a CU, and more
+@pytest.mark.parametrize("op", OPS)
+@by_type
+@pytest.mark.parametrize("rows,dim", [(2, 32768), (2, 32769), (3, 40001), (256, 6144), (256, 6145), (257, 12288),
+                                      (257, 12289), (300, 24577)])
+def test_quantize_shapes(dev, rows, dim, kind, op):
+    rng = np.random.default_rng(rows + dim + kind)
+    x, u = (rounded(3 * rng.standard_normal((rows, dim), dtype=np.float32), kind) for _ in range(2))
+    q, sc = torch.full((rows, dim), 99, dtype=torch.int8, device=dev), up_f32(np.full(rows, 9))
+    K.quantize_i8(q, sc, dev_rows(x, kind), None if op is None else dev_rows(u, kind), dim, rows, op or 0, kind)
+    quant_check(x if op is None else glu64(x, u, op), q, sc, (rows, dim, NAMES[kind], op))
+
+
+@by_type
+@pytest.mark.parametrize("rows,dim", [(256, 6144), (257, 6145), (256, 12289)])
+def test_norm_shapes(dev, rows, dim, kind):
+    for fmt in (ROWS_Q8_K, ROWS_I8):
+        n = Norm(rows, dim, kind)
+        a = n.arrays(fmt)
+        n.call(a, fmt)
+        n.check(a[3], a[2], a[0], a[1], fmt)
