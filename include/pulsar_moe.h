@@ -182,8 +182,9 @@ int pulsar_quantize_i8(void *q, void *scales, const void *x, const void *up, uin
  * sum, times the token's scale, times the channel's: a rounding to f32 each, as for bias,
  * activation and residual; one to `type` at the end. residual may be out itself, at the
  * same stride; any other overlap of out with an operand is refused. x_stride and w_stride
- * <= 2^23, out_stride and res_stride < 2^32. Rows on a 16-byte boundary (base and stride) run
- * fastest. */
+ * <= 2^23, out_stride and res_stride < 2^32, n_tok and out_dim < 2^31 (2^31 tiles of 128
+ * tokens x 128 channels are refused). Rows of whole 16 bytes on 16-byte boundaries (base,
+ * stride and in_dim) run fastest. */
 int pulsar_matmul_i8(void *out, const void *w, const void *w_scales, const void *x,
                      const void *x_scales, const void *bias, const void *residual,
                      uint32_t in_dim, uint32_t out_dim, uint32_t n_tok, uint32_t act,

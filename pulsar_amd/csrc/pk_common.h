@@ -30,6 +30,15 @@ static inline int launch_ok(const char *what) {
     return 0;
 }
 
+// A grid of n blocks (n < 2^31; the first axis a multiple of `unit`) and a block's index in
+// it, which may pass n. An axis holds fewer than 2^32 threads: of more, the launch leaves
+// out what is past them, without an error.
+static inline dim3 grid_of(uint64_t n, uint32_t unit = 1) {
+    const uint64_t y = (n + (1u << 21) - 1u) >> 21, x = ((n + y - 1u) / y + unit - 1u) / unit * unit;
+    return dim3((uint32_t)x, (uint32_t)y);
+}
+PK_DEV uint32_t block_index() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 static inline int reject(const char *what) {
     fprintf(stderr, "pulsar-kernels: %s: invalid arguments\n", what);
     return 0;

@@ -11,7 +11,7 @@ namespace pk {
 // it is as fast or 3% slower).
 template <uint32_t TYPE, uint32_t T>
 __global__ __launch_bounds__(256) void i8_lane_kernel(I8Args a) {
-    const uint32_t lane = threadIdx.x & 63u, r = blockIdx.x * 4u + (threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63u, r = block_index() * 4u + (threadIdx.x >> 6);
     if (r >= a.out_dim) return;  // wave-uniform
     const uint8_t *w = a.w + r * a.w_stride;
     int32_t acc[T] = {};
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void i8_lane_kernel(I8Args a) {
 }
 template <uint32_t TYPE, uint32_t T>
 static int launch_i8_lane(const I8Args &a) {
-    hipLaunchKernelGGL((i8_lane_kernel<TYPE, T>), dim3((a.out_dim + 3u) / 4u), dim3(256), 0, pk::stream(), a);
+    hipLaunchKernelGGL((i8_lane_kernel<TYPE, T>), grid_of((a.out_dim + 3u) / 4u), dim3(256), 0, pk::stream(), a);
     return launch_ok("matmul_i8 launch");
 }
 
@@ -64,10 +64,10 @@ int launch_i8(const I8Args &a) {
     // time grows with its tokens and channels, and a tile's reads for each product fall
     // with them. Of 411 shapes (1 to 8192 tokens, 64 to 28672 rows and 64 to 16384 columns)
     // the fastest of 15 tiles is missed by 1.6% on average, by more than 10% in 18.
-    // 16 x 16, 32 x 32, 32 x 64, 64 x 64, 64 x 128, 128 x 128, 128 x 256, 256 x 256, us: 16 tokens
-    // 4096 x 4096 5.9 / 6.2 / 6.9 / 9 / 11 / 15 / 24 / 52; 256 tokens 35 / 13 / 10.8 / 10.5 / 11.9 /
-    // 16 / 25 / 52; 1024 tokens 140 / 52 / 39 / 29 / 25 / 19 / 26 / 54; 4096 tokens x 4096 x 14336
-    // 1640 / 560 / 440 / 392 / 352 / 274 / 210 / 200
+    // us of 16 x 16, 32 x 32, 32 x 64, 64 x 64, 64 x 128, 128 x 128, 128 x 256, 256 x 256, 4096
+    // channels, 4096 values: 16 tokens 5.9 / 6.2 / 7.0 / 9.0 / 10.9 / 14 / 21 / 45; 256 tokens
+    // 50 / 20 / 13.2 / 10.1 / 11.6 / 14.6 / 22 / 46; 1024 tokens 206 / 74 / 47 / 28 / 24 / 19 / 24 /
+    // 47; 4096 tokens of 14336 values 1650 / 820 / 615 / 398 / 360 / 259 / 211 / 200
 #define PK_I8_TRY(...)                                    \
     do {                                                  \
         using T = I8Tile<__VA_ARGS__>;                    \
@@ -78,17 +78,17 @@ int launch_i8(const I8Args &a) {
     // wider tile takes as long
     const bool split = a.in_dim > 7u * 128u;
     if (!whole) {
-        // rows at any byte: the words of a step go through registers, which costs 1.3 to
-        // 2.5 times the time (130 tokens, 5001 x 2047 against 5008 x 2048: 11.0 / 6.6 us; 1023
-        // tokens 4095 x 4090 / 4096 x 4096: 37 / 19)
+        // rows at any byte: the words of a step go through registers, which costs 1.4 to
+        // 2.2 times the time (16 tokens 4095 x 4090 against 4096 x 4096: 8.4 / 6.0 us; 130 tokens
+        // 5001 x 2047 / 5008 x 2048: 11.9 / 6.9; 1023 tokens 4095 x 4090 / 4096 x 4096: 44 / 20)
         if (split) PK_I8_TRY(16, 16, 16, 1, 1, 8, 128, 2, false);
         PK_I8_TRY(16, 64, 64, 2, 4, 1, 128, 4, false);
         PK_I8_TRY(16, 64, 128, 2, 4, 1, 128, 4, false);
         return launch_i8_tile<TYPE, I8Tile<32, 128, 128, 4, 2, 1, 128, 2, false>>(a);
     }
     if (split) PK_I8_TRY(16, 16, 16, 1, 1, 8, 128, 4, true);
-    // two of 32 x 32: of long rows four groups take a part each (4096 x 4096, 48 tokens
-    // 6.6 against 7.3 us), for short ones joining them costs more (1024 x 256: 3.6 / 3.2)
+    // two of 32 x 32: of long rows four groups take a part each (4096 channels, 48 tokens of
+    // 4096 values 6.5 against 8.6 us), for short ones joining them costs more (1024: 4.0 / 3.7)
     if (a.in_dim > 1024u)
         PK_I8_TRY(16, 32, 32, 2, 1, 4, 128, 4, true);
     else

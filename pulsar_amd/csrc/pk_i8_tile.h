@@ -131,7 +131,7 @@ __global__ __launch_bounds__(T::kThreads) void i8_tile_kernel(I8Args a, uint32_t
     // XCD x (blocks x, x + 8, ...) takes the x-th eighth of the items; 4 channel tiles by
     // all token tiles are one run of them, channels first: what an XCD works on at a time
     // is about as many tokens as channels
-    const uint32_t item = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const uint32_t block = block_index(), item = (block & 7u) * (gridDim.x * gridDim.y >> 3) + (block >> 3);
     if (item >= n_item) return;  // block-uniform
     const uint32_t panel = item / (4u * n_tt), in_panel = item - panel * 4u * n_tt;
     const uint32_t width = n_rt - 4u * panel < 4u ? n_rt - 4u * panel : 4u;
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(T::kThreads) void i8_tile_kernel(I8Args a, uint32_t
     }
 }
 
-// Tiles of the shape; 0: more than a grid takes
+// Tiles of the shape
 template <typename T>
 static uint64_t i8_items(const I8Args &a) {
     return (uint64_t)((a.n_tok + T::BM - 1u) / T::BM) * ((a.out_dim + T::BN - 1u) / T::BN);
@@ -416,8 +416,8 @@ static uint64_t i8_items(const I8Args &a) {
 template <uint32_t TYPE, typename T>
 static int launch_i8_tile(const I8Args &a) {
     const uint64_t n = i8_items<T>(a);
-    if (n > 0x7ffffff0ull) return reject("matmul_i8 (size)");
-    hipLaunchKernelGGL((i8_tile_kernel<TYPE, T>), dim3((uint32_t)((n + 7u) & ~7ull)), dim3(T::kThreads), 0, pk::stream(), a,
+    if (n >> 31) return reject("matmul_i8 (size)");
+    hipLaunchKernelGGL((i8_tile_kernel<TYPE, T>), grid_of(n, 8u), dim3(T::kThreads), 0, pk::stream(), a,
                        (a.n_tok + T::BM - 1u) / T::BM, (a.out_dim + T::BN - 1u) / T::BN, (uint32_t)n);
     return launch_ok("matmul_i8 tile launch");
 }

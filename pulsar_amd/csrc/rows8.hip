@@ -72,7 +72,7 @@ struct NormArgs {
     const raw *x, *residual;
     const float *gain;
     uint64_t x_stride, res_stride, sum_stride, q_stride;
-    uint32_t dim, format;
+    uint32_t dim, n_rows, format;
     float eps;
 };
 
@@ -153,7 +153,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
     __shared__ RowStats lds;
     const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = block_index();
+    if (row >= a.n_rows) return;  // block-uniform
     const bool blocks = a.format == PULSAR_ROWS_Q8_K;
     auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
     double ss = 0.0;
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs<TYPE> a) {
     constexpr uint32_t V = kLane<TYPE>;
     __shared__ RowStats lds;
     const uint32_t step = V * blockDim.x;
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = block_index();
+    if (row >= a.n_rows) return;  // block-uniform
     const bool blocks = a.format == PULSAR_ROWS_Q8_K;
     double ss = 0.0, p[V];
     uint64_t row_top = 0u;
@@ -283,7 +285,7 @@ struct QuantArgs {
     float *scales;
     const raw *x, *up;  // up NULL: x as it is
     uint64_t x_stride, up_stride, q_stride;
-    uint32_t dim, act_op;
+    uint32_t dim, n_rows, act_op;
 };
 
 template <uint32_t TYPE, uint32_t V>
@@ -304,7 +306,7 @@ template <uint32_t TYPE>
 PK_DEV void quantize_row(const QuantArgs<TYPE> &a, RowStats &lds) {
     constexpr uint32_t V = kLane<TYPE>;
     const uint32_t step = V * blockDim.x;
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = block_index();
     double v[V], none = 0.0;
     uint64_t top = 0u;
     for (uint32_t c0 = V * threadIdx.x; c0 < a.dim; c0 += step) {
@@ -327,6 +329,7 @@ PK_DEV void quantize_row(const QuantArgs<TYPE> &a, RowStats &lds) {
 template <uint32_t TYPE>
 __global__ __launch_bounds__(1024) void quantize_i8_long_kernel(QuantArgs<TYPE> a) {
     __shared__ RowStats lds;
+    if (block_index() >= a.n_rows) return;  // block-uniform
     quantize_row(a, lds);
 }
 
@@ -337,7 +340,8 @@ __global__ __launch_bounds__(1024) void quantize_i8_kernel(QuantArgs<TYPE> a) {
     __shared__ RowStats lds;
     const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = block_index();
+    if (row >= a.n_rows) return;  // block-uniform
     auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
     float x[NB][V];
     double none = 0.0;
@@ -403,7 +407,8 @@ __global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
     __shared__ RowStats lds, lds64;
     const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = block_index();
+    if (row >= a.n_rows) return;  // block-uniform
     auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
     auto whole = [&](uint32_t j) { return 64u * V * (wave + waves * j + 1u) <= a.dim; };  // wave-uniform
     const raw *x = a.x + row * a.x_stride, *up = a.up + row * a.up_stride;
@@ -535,9 +540,9 @@ static int launch_norm(void *q, void *scales, void *y, void *sum, const void *x,
     typedef typename Elem<TYPE>::raw raw;
     const NormArgs<TYPE> a = {(uint8_t *)q, (float *)scales, (raw *)y, (raw *)sum, (const raw *)x,
                               (const raw *)residual, (const float *)gain, x_stride, res_stride, sum_stride, q_stride,
-                              dim, format, eps};
+                              dim, n_rows, format, eps};
     const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kNormChunks<TYPE>);
-    const dim3 grid(n_rows), block(64u * s.waves);
+    const dim3 grid = grid_of(n_rows), block(64u * s.waves);
     if (s.chunks == 1u)
         hipLaunchKernelGGL((norm_kernel<TYPE, 1>), grid, block, 0, pk::stream(), a);
     else if (s.chunks == 2u)
@@ -554,9 +559,9 @@ static int launch_quantize(void *q, void *scales, const void *x, const void *up,
                            uint32_t act_op, uint64_t x_stride, uint64_t up_stride, uint64_t q_stride) {
     typedef typename Elem<TYPE>::raw raw;
     const QuantArgs<TYPE> a = {(uint8_t *)q, (float *)scales, (const raw *)x, (const raw *)up, x_stride, up_stride,
-                               q_stride, dim, act_op};
+                               q_stride, dim, n_rows, act_op};
     const RowShape s = row_shape((dim + 64u * kLane<TYPE> - 1u) / (64u * kLane<TYPE>), n_rows, kQuantChunks<TYPE>);
-    const dim3 grid(n_rows), block(64u * s.waves);
+    const dim3 grid = grid_of(n_rows), block(64u * s.waves);
 #define PK_QUANT_NB(NB)                                                                        \
     do {                                                                                       \
         if (up)                                                                                \

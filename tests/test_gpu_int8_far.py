@@ -139,3 +139,36 @@ def test_same_bits_every_time(dev, rows, cols, T):
         got = down(out)
         first = got if first is None else first
         assert np.array_equal(first.view(np.uint32), got.view(np.uint32))
+
+
+def test_more_threads_than_an_axis_holds(dev):
+    """2^26 waves and more: rows of one value, channels of one token."""
+    n = 2**26 + 5003
+    x, q, sc = torch.ones((n, 1), device=dev), torch.zeros((n, 1), dtype=torch.int8, device=dev), zeros_f32(n)
+    K.rms_norm_q8(q, sc, None, None, x, None, up_f32(np.full(1, 2.0)), 1, n, 0.0, TYPE_F32, ROWS_I8)
+    torch.cuda.synchronize()
+    assert (q == 127).all() and (sc == float(np.float32(2 / 127))).all()
+    q.zero_()
+    for up in (None, x):
+        torch.cuda.synchronize()
+        K.quantize_i8(q, sc, x, up, 1, n)
+        torch.cuda.synchronize()
+        assert (q == 127).all()
+        q.zero_()
+    w, ws, out = torch.ones((n, 3), dtype=torch.int8, device=dev), torch.ones(n, device=dev), zeros_f32((2, n))
+    x = torch.tensor([[1, 2, 3], [4, 5, -6]], dtype=torch.int8, device=dev)
+    torch.cuda.synchronize()
+    for T in (1, 2):
+        K.matmul_i8(out, w, ws, x, up_f32(np.ones(2)), None, None, 3, n, T)
+        torch.cuda.synchronize()
+        assert (out[0] == 6).all() and (out[1] == (3 if T == 2 else 0)).all()
+
+
+# tokens times the tiles' threads past 2^32: rows at any byte, and whole pieces
+@pytest.mark.parametrize("T,cols", [(2**30 + 1000, 1), (2**31 - 1, 16)])
+def test_more_tiles_than_an_axis_holds(dev, T, cols):
+    x, sx, out = torch.ones((T, cols), dtype=torch.int8, device=dev), torch.ones(T, device=dev), zeros_f32((T, 1))
+    torch.cuda.synchronize()
+    K.matmul_i8(out, torch.ones((1, cols), dtype=torch.int8, device=dev), up_f32(np.ones(1)), x, sx, None, None, cols, 1, T)
+    torch.cuda.synchronize()
+    assert (out == cols).all()

@@ -236,3 +236,9 @@ def test_refuses_host_tensors():
     for call, name in ((norm, "x"), (norm, "gain"), (quant, "x"), (product, "out"), (product, "w_scales")):
         with pytest.raises(ValueError, match="host tensor"):
             call(**{name: t})
+
+
+def test_product_refuses_more_tiles_than_a_grid(capfd):
+    """2^27 tokens by 2^31 - 1 channels, out where no other array is."""
+    call = lambda: product(out=1 << 62, residual=0, out_dim=2**31 - 1, n_tok=2**27, type=TYPE_BF16)  # noqa: E731
+    assert "matmul_i8 (size)" in said(capfd, call)
