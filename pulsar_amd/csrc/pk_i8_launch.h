@@ -79,11 +79,17 @@ int launch_i8(const I8Args &a) {
     const bool split = a.in_dim > 7u * 128u;
     if (!whole) {
         // rows at any byte: the words of a step go through registers, which costs 1.4 to
-        // 2.2 times the time (16 tokens 4095 x 4090 against 4096 x 4096: 8.4 / 6.0 us; 130 tokens
-        // 5001 x 2047 / 5008 x 2048: 11.9 / 6.9; 1023 tokens 4095 x 4090 / 4096 x 4096: 44 / 20)
+        // 1.9 times the time (16 tokens 4095 x 4090 against 4096 x 4096: 8.6 / 6.0 us; 130 tokens
+        // 5001 x 2047 / 5008 x 2048: 10.2 / 6.9; 1023 tokens 4095 x 4090 / 4096 x 4096: 35 / 21;
+        // 4095 tokens 122 / 65). Two groups of 32 x 32, and 16 waves for one round of tiles of
+        // 128 x 128, 8 for more (40 tokens 2881 x 2049 6.5 us, 4 groups 7.9; 1023 tokens 4095 x
+        // 4090 32, 8 waves 42; 4095 tokens 126, 16 waves 145)
         if (split) PK_I8_TRY(16, 16, 16, 1, 1, 8, 128, 2, false);
+        PK_I8_TRY(16, 32, 32, 2, 2, 2, 128, 4, false);
+        PK_I8_TRY(16, 32, 64, 2, 2, 2, 128, 4, false);
         PK_I8_TRY(16, 64, 64, 2, 4, 1, 128, 4, false);
         PK_I8_TRY(16, 64, 128, 2, 4, 1, 128, 4, false);
+        PK_I8_TRY(16, 128, 128, 4, 4, 1, 128, 4, false);
         return launch_i8_tile<TYPE, I8Tile<32, 128, 128, 4, 2, 1, 128, 2, false>>(a);
     }
     if (split) PK_I8_TRY(16, 16, 16, 1, 1, 8, 128, 4, true);

@@ -145,12 +145,11 @@ __global__ __launch_bounds__(T::kThreads) void i8_tile_kernel(I8Args a, uint32_t
     const uint8_t *xb = a.x + t0 * a.x_stride, *wb = a.w + r0 * a.w_stride;
     const uint32_t xs = (uint32_t)a.x_stride, ws = (uint32_t)a.w_stride;  // at most 2^23: offsets of a tile fit 32 bits
     const uint32_t x_bytes = (nx - 1u) * xs + a.in_dim, w_bytes = (nw - 1u) * ws + a.in_dim;
-    // the byte of a step that the lane copies of the row of copy j
+    // the byte of a step that the lane copies of the row of copy j: with DMA, whose lanes
+    // land side by side, of the piece that belongs there; else a row's pieces in order
     constexpr uint32_t kPieces = T::KB / 16u;
-    auto piece_of = [&](uint32_t j) {
-        const uint32_t row = T::kRows * (in_group + T::kGroup * j) + lane / kPieces;
-        return 16u * ((lane % kPieces) ^ i8_slot_of<T::KB>(row));
-    };
+    auto slot_of = [&](uint32_t j) { return i8_slot_of<T::KB>(T::kRows * (in_group + T::kGroup * j) + lane / kPieces); };
+    auto piece_of = [&](uint32_t j) { return 16u * ((lane % kPieces) ^ (T::DMA ? slot_of(j) : 0u)); };
     // a copy's row; without bounds of their own (!DMA) rows behind the last are the last
     auto row_of = [&](uint32_t j, uint32_t n) {
         const uint32_t row = T::kRows * (in_group + T::kGroup * j) + lane / kPieces;
@@ -191,35 +190,40 @@ __global__ __launch_bounds__(T::kThreads) void i8_tile_kernel(I8Args a, uint32_t
         else
             copy_to_lds(st.w, from[j] + st.k, buffer + to_of(j));
     };
-    // Without DMA: a step's pieces as the words that each lies in, which the lane shifts:
-    // loads at odd bytes take the memory pipe longer. The buffers start and end with the
-    // words of the tile's first and last byte, so nothing is read but words that the rows
-    // are in, and a load needs no condition of its own
-    uint4 lo[T::DMA ? 1u : S][kCopies];
-    uint32_t hi[T::DMA ? 1u : S][kCopies];
+    // Without DMA: a step's pieces as the words that each starts in, which the lane shifts:
+    // loads at odd bytes take the memory pipe longer. What a piece has in the word behind
+    // its four is the next lane's first, for the last piece that of the row's next step,
+    // and a group's steps follow one another for that (130 tokens 5001 x 2047: 9.6 us, with
+    // loads of those words 11.1). The buffers start and end with the words of the tile's first and
+    // last byte, so nothing is read but words that the rows are in, and a load needs no
+    // condition of its own
+    const uint32_t n_it = ((a.in_dim + T::KB - 1u) / T::KB + T::WK - 1u) / T::WK;
+    uint4 words[T::DMA ? 1u : S][kCopies];
     const uint32_t x_odd = (uint32_t)(uintptr_t)xb & 3u, w_odd = (uint32_t)(uintptr_t)wb & 3u;
     const auto x_words = __builtin_amdgcn_make_buffer_rsrc((void *)(xb - x_odd), 0, (int)((x_bytes + x_odd + 3u) & ~3u), 0x00027000);
     const auto w_words = __builtin_amdgcn_make_buffer_rsrc((void *)(wb - w_odd), 0, (int)((w_bytes + w_odd + 3u) & ~3u), 0x00027000);
+    auto step_at = [&](uint32_t it) { return T::KB * (group * n_it + it); };
     auto fetch = [&](uint32_t h, uint32_t it) {
-        const uint32_t k = T::KB * (it * T::WK + group);
 #pragma unroll
         for (uint32_t j = 0; j < kCopies; j++) {
-            const uint32_t at = (from[j] + (j < T::kX ? x_odd : w_odd) + k) & ~3u;
-            const auto words = j < T::kX ? x_words : w_words;
-            lo[h][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(words, at, 0, 0));
-            hi[h][j] = __builtin_amdgcn_raw_buffer_load_b32(words, at + 16u, 0, 0);
+            const uint32_t at = (from[j] + (j < T::kX ? x_odd : w_odd) + step_at(it)) & ~3u;
+            words[h][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(j < T::kX ? x_words : w_words, at, 0, 0));
         }
     };
     auto put = [&](uint8_t *buf, uint32_t h, uint32_t it) {
-        const uint32_t k = T::KB * (it * T::WK + group);
+        static_assert(T::DMA || kPieces == 8u, "lanes of a row");
+        const uint32_t k = step_at(it);
 #pragma unroll
         for (uint32_t j = 0; j < kCopies; j++) {
-            uint4 v = shifted(lo[h][j], hi[h][j], (from[j] + (j < T::kX ? x_odd : w_odd)) & 3u);
+            const uint32_t beside = __builtin_amdgcn_update_dpp(0, (int)words[h][j].x, 0x101, 0xf, 0xf, true);  // lane + 1's
+            const uint32_t after = __builtin_amdgcn_update_dpp(0, (int)words[(h + 1u) % S][j].x, 0x117, 0xf, 0xf, true);  // lane - 7's
+            uint4 v = shifted(words[h][j], lane % 8u == 7u ? after : beside, (from[j] + (j < T::kX ? x_odd : w_odd)) & 3u);
             if (j < T::kX && k + T::KB > a.in_dim) {  // uniform; of the tokens alone, as above
                 const uint32_t at = k + piece_of(j);
                 v = first_bytes(v, at < a.in_dim ? a.in_dim - at : 0u);
             }
-            *(uint4 *)(buf + to_of(j) + 16u * lane) = v;
+            const uint32_t slot = (lane & ~7u) | ((lane & 7u) ^ slot_of(j < T::kX ? j : j - T::kX));
+            *(uint4 *)(buf + to_of(j) + 16u * slot) = v;
         }
     };
     auto barrier = [] {
@@ -266,7 +270,6 @@ __global__ __launch_bounds__(T::kThreads) void i8_tile_kernel(I8Args a, uint32_t
     };
     // copies of a step that are issued behind its wait, among the last slice's MFMAs
     constexpr uint32_t kBehind = kCopies - (((T::kSub - 1u) * kMfmas * kCopies + kSlots - 1u) / kSlots);
-    const uint32_t n_it = ((a.in_dim + T::KB - 1u) / T::KB + T::WK - 1u) / T::WK;
     if constexpr (T::DMA) {
 #pragma unroll
         for (uint32_t s = 0; s + 1u < S; s++) {

@@ -207,3 +207,27 @@ def test_dense_ffn(dev, T, hidden, ffn, kind):
         dots = int_dots(hmq, wd) * hmsc[:, None].astype(np.float64) * sd
         tol = 2.0**-24 * (3.1 * np.abs(dots) + 1.1 * np.abs(dots + hs)) + HALF[kind] * 1.01 * np.abs(dots + hs) + TINY[kind]
         assert (np.abs(host(out) - (dots + hs)) <= tol).all()
+
+
+# a shape for each kernel of rows at any byte, with row ends in every place of a word,
+# a 16-byte piece and a step of 128
+@pytest.mark.parametrize("rows,cols,T", [(700, 1501, 5), (512, 4099, 16), (500, 261, 40), (600, 1026, 33), (6000, 131, 60),
+                                         (5001, 1027, 61), (5001, 255, 130), (5000, 390, 200), (2049, 257, 1000),
+                                         (2048, 513, 1023), (2100, 642, 2100)])
+@pytest.mark.parametrize("x_at,w_at,x_pad,w_pad", [(0, 1, 1, 3), (1, 2, 2, 1), (2, 3, 3, 2), (3, 0, 0, 0), (0, 0, 4, 1)])
+def test_rows_at_any_byte(dev, rows, cols, T, x_at, w_at, x_pad, w_pad):
+    """Bytes between the rows are -128 and 127, and the arrays end with the last row."""
+    c = Case(rows, cols, T, TYPE_BF16)
+
+    def placed(a, at, pad, fill):
+        n = a.shape[0]
+        t = torch.full((at + (n - 1) * (cols + pad) + cols,), fill, dtype=torch.int8, device=dev)
+        v = t[at:].as_strided((n, cols), (cols + pad, 1))
+        v.copy_(i8(a))
+        return v
+
+    x, w = placed(c.x, x_at, x_pad, -128), placed(c.w, w_at, w_pad, 127)
+    out = out_of(c)
+    K.matmul_i8(out, w, up_f32(c.sw), x, up_f32(c.sx), up_f32(c.bias), dev_rows(c.res, c.kind), cols, rows, T, EPI_SILU,
+                c.kind, cols + w_pad, cols + x_pad)
+    c.check(host(out), True, EPI_SILU, True)
