@@ -14,6 +14,13 @@
 // WM x WN waves share a step's tokens and channels; WK such groups split the steps among
 // them, for sizes whose tiles would leave much of the chip idle, and add their sums in
 // LDS at the end.
+//
+// Measured: 4096 tokens through 4096 x 14336, bias and residual, bf16, 209 us, 2300 T
+// operations a second; 8192 tokens of 8192 x 8192 457 us, 2400. What bounds them is power:
+// with random bytes the card runs at 1.76 GHz, with zeros at 2.46 and takes 168 of the 200 us
+// without an epilogue; the MFMAs alone, their operands in registers, reach 3500 to 4000 T on random
+// bytes. Start and end of a block take some 10 us. 16 tokens of 8192 x 4096 read 34 MB in 8.4
+// us, 4.1 TB/s: a launch and HBM.
 #pragma once
 
 #include "pk_i8.h"

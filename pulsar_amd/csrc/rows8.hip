@@ -7,8 +7,8 @@
 // registers and is written once. The norm needs one exchange between the waves: its root
 // divides every value of the row alike, so codes and the largest size are those of s *
 // gain, known without it. Sums, products and codes in 64 bits cost about what the bytes
-// do: a value is 5 to 17 bytes of traffic and some 20 operations, most of them at the rate
-// of f32's. Measured (GB/s of what has to move): norm of 8192 rows of 4096 bf16 values to
+// do: a value of a norm is 7 to 17 bytes of traffic and 35 instructions, most of them at the
+// rate of f32's. Measured (GB/s of what has to move): norm of 8192 rows of 4096 bf16 values to
 // int8 59 us (3970), to q8_K with y 70 (4390), of 2048 rows of f32 32 (4490), quantized as
 // they are 20 (5000), combined by glu first 43 (3900).
 #include "pk_elem.h"
@@ -396,10 +396,10 @@ PK_DEV float min3(float a, float b, float c) { return __builtin_elementwise_mini
 // off by 2^-20, those that may be the row's largest are combined again in 64 bits, and
 // those whose code argument (up to 127: off by 2^-13) lies within 2^-12 of a half, one in
 // 2000. The common way only asks a lane's largest and its nearest to a half; a lane with
-// some looks for which. Bound by its instructions, two transcendental ones among them: of
-// 8192 rows of 4096 bf16 values the pipes are busy most of 43 us (59 with a mask kept for
-// every value), 3900 GB/s; 4096 rows of 14336 84 us, 3490 GB/s (175 with every value
-// combined in 64 bits).
+// some looks for which. 4096 rows of 14336 bf16 values take 84 us, 3490 GB/s (175 with
+// every value combined in 64 bits); the vector pipes are busy 54% of it, with 31
+// instructions a value, two of them transcendental; waves wait 63% of their time for
+// memory or one another. 8192 rows of 4096: 43 us, 3900 GB/s.
 template <uint32_t TYPE, uint32_t NB>
 __global__ __launch_bounds__(1024) void glu_i8_kernel(QuantArgs<TYPE> a) {
     constexpr uint32_t V = kLane<TYPE>;
