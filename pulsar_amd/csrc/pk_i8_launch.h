@@ -83,12 +83,14 @@ int launch_i8(const I8Args &a) {
         // 5001 x 2047 / 5008 x 2048: 10.2 / 6.9; 1023 tokens 4095 x 4090 / 4096 x 4096: 35 / 21;
         // 4095 tokens 122 / 65). Two groups of 32 x 32, and 16 waves for one round of tiles of
         // 128 x 128, 8 for more (40 tokens 2881 x 2049 6.5 us, 4 groups 7.9; 1023 tokens 4095 x
-        // 4090 32, 8 waves 42; 4095 tokens 126, 16 waves 145)
+        // 4090 32, 8 waves 42; 4095 tokens 126, 16 waves 145). Up to 64 tokens rounds of 64 x
+        // 128, not of 128 x 128 (8 tokens 151935 x 4095 138 / 157; 64 tokens 60001 x 2047 41 / 42)
         if (split) PK_I8_TRY(16, 16, 16, 1, 1, 8, 128, 2, false);
         PK_I8_TRY(16, 32, 32, 2, 2, 2, 128, 4, false);
         PK_I8_TRY(16, 32, 64, 2, 2, 2, 128, 4, false);
         PK_I8_TRY(16, 64, 64, 2, 4, 1, 128, 4, false);
-        PK_I8_TRY(16, 64, 128, 2, 4, 1, 128, 4, false);
+        using Wide = I8Tile<16, 64, 128, 2, 4, 1, 128, 4, false>;
+        if (i8_items<Wide>(a) <= kI8Slots || a.n_tok <= 64u) return launch_i8_tile<TYPE, Wide>(a);
         PK_I8_TRY(16, 128, 128, 4, 4, 1, 128, 4, false);
         return launch_i8_tile<TYPE, I8Tile<32, 128, 128, 4, 2, 1, 128, 2, false>>(a);
     }
@@ -100,8 +102,14 @@ int launch_i8(const I8Args &a) {
     else
         PK_I8_TRY(16, 32, 32, 2, 2, 1, 128, 4, true);
     PK_I8_TRY(16, 32, 64, 2, 2, 2, 128, 4, true);
-    PK_I8_TRY(32, 64, 64, 2, 2, 1, 128, 4, true);
+    // many channels of few tokens: rounds of a tile without room for many more tokens (16
+    // tokens of 4096 values, 151936 channels 126 us, 128 x 256 144; 64 tokens 138 / 151; of 23
+    // shapes with up to 32 tokens the fastest tile is missed by 4%, without this by 9%)
+    if (a.n_tok <= 32u) return launch_i8_tile<TYPE, I8Tile<16, 32, 32, 2, 2, 1, 128, 4, true>>(a);
+    using Square = I8Tile<32, 64, 64, 2, 2, 1, 128, 4, true>;
+    if (i8_items<Square>(a) <= kI8Slots) return launch_i8_tile<TYPE, Square>(a);
     PK_I8_TRY(16, 64, 128, 2, 4, 1, 128, 4, true);
+    if (a.n_tok <= 64u) return launch_i8_tile<TYPE, Square>(a);
     PK_I8_TRY(16, 128, 128, 4, 2, 1, 128, 4, true);
     using Half = I8Tile<32, 128, 256, 2, 4, 1, 128, 3, true>;
     using Widest = I8Tile<16, 256, 256, 2, 4, 1, 64, 4, true>;

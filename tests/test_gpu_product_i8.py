@@ -231,3 +231,14 @@ def test_rows_at_any_byte(dev, rows, cols, T, x_at, w_at, x_pad, w_pad):
     K.matmul_i8(out, w, up_f32(c.sw), x, up_f32(c.sx), up_f32(c.bias), dev_rows(c.res, c.kind), cols, rows, T, EPI_SILU,
                 c.kind, cols + w_pad, cols + x_pad)
     c.check(host(out), True, EPI_SILU, True)
+
+
+# more channels than a round of the tiles that fit few tokens
+@pytest.mark.parametrize("kind", [TYPE_F32, TYPE_BF16], ids=NAMES.get)
+@pytest.mark.parametrize("rows,cols,T", [(17000, 304, 3), (17000, 1040, 32), (33000, 144, 33), (33000, 272, 64),
+                                         (33000, 144, 65), (33000, 143, 9), (33000, 77, 64), (33000, 45, 65)])
+def test_many_channels(dev, rows, cols, T, kind):
+    c = Case(rows, cols, T, kind)
+    out = out_of(c)
+    K.matmul_i8(out, *c.buffers(), up_f32(c.bias), dev_rows(c.res, kind), cols, rows, T, EPI_RELU, kind)
+    c.check(host(out), True, EPI_RELU, True)
