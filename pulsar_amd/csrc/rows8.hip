@@ -157,6 +157,14 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
     if (row >= a.n_rows) return;  // block-uniform
     const bool blocks = a.format == PULSAR_ROWS_Q8_K;
     auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
+    // f of how many of the lane's values of chunk j are there: a constant where all lanes'
+    // are, whose loads then need no masks (2048 rows of 14336 f32 values 96 us against 104)
+    auto with_count = [&](uint32_t j, auto f) {
+        if (64u * V * (wave + waves * j + 1u) <= a.dim)  // wave-uniform
+            f(V);
+        else
+            f(inside<V>(first(j), a.dim));
+    };
     double ss = 0.0;
     uint64_t top[NB], row_top = 0u;
     // held over the exchange in the rows' type, a quarter of the products' registers: two
@@ -165,15 +173,16 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
     {
         float s[NB][V];
 #pragma unroll
-        for (uint32_t j = 0; j < NB; j++) norm_load(a, row, first(j), inside<V>(first(j), a.dim), s[j]);
+        for (uint32_t j = 0; j < NB; j++) with_count(j, [&](uint32_t n) { norm_load(a, row, first(j), n, s[j]); });
 #pragma unroll
         for (uint32_t j = 0; j < NB; j++) {
-            const uint32_t n = inside<V>(first(j), a.dim);
-            double p[V];
+            with_count(j, [&](uint32_t n) {
+                double p[V];
 #pragma unroll
-            for (uint32_t k = 0; k < V; k++) held[j][k] = Elem<TYPE>::down(s[j][k]);  // exact
-            if (a.sum) store_row(a.sum + row * a.sum_stride + first(j), n, held[j]);
-            top[j] = norm_products(a, first(j), n, s[j], p, ss);
+                for (uint32_t k = 0; k < V; k++) held[j][k] = Elem<TYPE>::down(s[j][k]);  // exact
+                if (a.sum) store_row(a.sum + row * a.sum_stride + first(j), n, held[j]);
+                top[j] = norm_products(a, first(j), n, s[j], p, ss);
+            });
         }
     }
 #pragma unroll
@@ -191,14 +200,15 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
 #pragma unroll
     for (uint32_t j = 0; j < NB; j++) {
         if (64u * V * (wave + waves * j) >= a.dim) break;  // wave-uniform
-        const uint32_t n = inside<V>(first(j), a.dim);
-        float g[V];
-        double p[V];
-        load_row<PULSAR_TYPE_F32>(a.gain + first(j), n, g);
+        with_count(j, [&](uint32_t n) {
+            float g[V];
+            double p[V];
+            load_row<PULSAR_TYPE_F32>(a.gain + first(j), n, g);
 #pragma unroll
-        for (uint32_t k = 0; k < V; k++) p[k] = (double)Elem<TYPE>::up(held[j][k]) * (double)g[k];
-        norm_put(a, row, first(j), n, p, root, blocks ? top[j] : row_top,
-                 blocks ? code_factor(__builtin_bit_cast(double, top[j])) : row_factor);
+            for (uint32_t k = 0; k < V; k++) p[k] = (double)Elem<TYPE>::up(held[j][k]) * (double)g[k];
+            norm_put(a, row, first(j), n, p, root, blocks ? top[j] : row_top,
+                     blocks ? code_factor(__builtin_bit_cast(double, top[j])) : row_factor);
+        });
     }
     if (a.scales && threadIdx.x == 0u)
         a.scales[row] = (float)(__builtin_bit_cast(double, row_top) * root * (1.0 / 127.0));
@@ -522,7 +532,7 @@ static RowShape row_shape(uint32_t n_chunk, uint32_t n_rows, uint32_t most) {
     return {(n_chunk + nb - 1u) / nb, nb};
 }
 // Chunks of a wave at most: 16 values a lane in a norm, whose products are of 64 bits
-// (with 32, 2048 rows of 14336 f32 values take 151 us against 133), 32 in the quantizers
+// (with 32, 2048 rows of 14336 f32 values took 151 us against 133), 32 in the quantizers
 template <uint32_t TYPE>
 constexpr uint32_t kNormChunks = 16u / kLane<TYPE>;
 template <uint32_t TYPE>
