@@ -363,6 +363,7 @@ __global__ __launch_bounds__(T::kThreads) void i8_tile_kernel(I8Args a, uint32_t
         if (a.residual) {
 #pragma unroll
             for (uint32_t i = 0; i < kOwn; i++) {
+                if (!any(i)) continue;  // tokens behind the tile's, and behind the array's end
                 const raw *from_row = residual + (p * T::kSliceTok + i * T::WK * kTok) * a.res_stride;
                 if (whole)
                     load_row4<TYPE>(from_row, 4u, res[i]);

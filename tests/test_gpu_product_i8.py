@@ -242,3 +242,18 @@ def test_many_channels(dev, rows, cols, T, kind):
     out = out_of(c)
     K.matmul_i8(out, *c.buffers(), up_f32(c.bias), dev_rows(c.res, kind), cols, rows, T, EPI_RELU, kind)
     c.check(host(out), True, EPI_RELU, True)
+
+
+# tiles whose groups outnumber the parts of their sums, all tokens and channels of a tile there
+@pytest.mark.parametrize("kind", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("rows,cols,T", [(256, 1024, 160), (256, 1025, 160), (1024, 2048, 224), (1030, 2048, 200),
+                                         (64, 4096, 16), (2048, 2064, 32)])
+def test_residual_that_ends_with_its_memory(dev, rows, cols, T, kind):
+    """Residual and output in the last bytes of allocations of whole pages."""
+    c = Case(rows, cols, T, kind)
+    res, out = (torch.zeros(2**25 // TORCH[kind].itemsize, dtype=TORCH[kind], device=dev)[-T * rows:].view(T, rows)
+                for _ in range(2))
+    res.copy_(dev_rows(c.res, kind))
+    bufs, bias = c.buffers(), up_f32(c.bias)
+    K.matmul_i8(out, *bufs, bias, res, cols, rows, T, EPI_GELU, kind)
+    c.check(host(out), True, EPI_GELU, True)
