@@ -257,3 +257,13 @@ def test_residual_that_ends_with_its_memory(dev, rows, cols, T, kind):
     bufs, bias = c.buffers(), up_f32(c.bias)
     K.matmul_i8(out, *bufs, bias, res, cols, rows, T, EPI_GELU, kind)
     c.check(host(out), True, EPI_GELU, True)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("rows,cols,T", [(2050, 2048, 200), (2050, 2064, 200), (4096, 4112, 256), (4096, 2064, 192)])
+def test_two_groups_of_64(dev, rows, cols, T, kind):
+    """On both sides of the row length from which two groups share a 64 x 64 tile."""
+    c = Case(rows, cols, T, kind)
+    out = out_of(c)
+    K.matmul_i8(out, *c.buffers(), up_f32(c.bias), dev_rows(c.res, kind), cols, rows, T, EPI_GELU, kind)
+    c.check(host(out), True, EPI_GELU, True)
