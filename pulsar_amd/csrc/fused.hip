@@ -39,12 +39,13 @@ __global__ __launch_bounds__(256) void router_logits_q8_kernel(
         float *__restrict__ logits, pulsar_block_q8_K *__restrict__ xq, const float *__restrict__ x,
         const float *__restrict__ w, const float *__restrict__ bias, uint32_t in_dim, uint32_t n_expert,
         uint32_t n_tok, uint32_t gemv_blocks, uint32_t nb, uint32_t rb_log2) {
-    if (blockIdx.x < gemv_blocks) {
+    const uint32_t block = block_index();
+    if (block < gemv_blocks) {
         gemv_block<TG>(logits, w, x, bias, in_dim, n_expert, n_tok,
-                       gemv_item(blockIdx.x, n_expert, gemv_blocks / n_expert, rb_log2));
+                       gemv_item(block, n_expert, gemv_blocks / n_expert, rb_log2));
         return;
     }
-    const uint32_t gblk = (blockIdx.x - gemv_blocks) * 4u + (threadIdx.x >> 6);
+    const uint32_t gblk = (block - gemv_blocks) * 4u + (threadIdx.x >> 6);
     if (gblk >= n_tok * nb) return;  // whole wave
     const uint32_t row = gblk / nb, b = gblk - row * nb;
     quantize_block_wave<4u, 260u>(x + (uint64_t)row * in_dim, in_dim, b, (uint8_t *)(xq + gblk));
@@ -340,15 +341,15 @@ using namespace pk;
 
 extern "C" int pulsar_router_logits_q8(void *logits, void *xq, const void *x, const void *w_r, const void *bias,
                                        uint32_t in_dim, uint32_t n_expert, uint32_t n_tok) {
-    if (!logits || !xq || !x || !w_r || in_dim == 0 || n_expert == 0 || n_tok == 0)
+    if (!logits || !xq || !x || !w_r || in_dim == 0 || in_dim > kMaxRow || n_expert == 0 || n_tok == 0)
         return reject("router logits q8");
     const uint32_t tg = n_tok == 1u ? 1u : 2u;
-    const uint64_t work = (uint64_t)n_expert * ((n_tok + tg - 1u) / tg);
+    const uint64_t work = (uint64_t)n_expert * (((uint64_t)n_tok + tg - 1u) / tg);
     const uint32_t nb = (in_dim + 255u) / 256u;
     const uint64_t qblocks = ((uint64_t)n_tok * nb + 3u) / 4u;
     const uint64_t gemv_blocks = work;
-    if (gemv_blocks + qblocks > 0x7fffffffull) return reject("router logits q8 (size)");
-    const dim3 grid((uint32_t)(gemv_blocks + qblocks));
+    if ((gemv_blocks + qblocks) >> 31) return reject("router logits q8 (size)");
+    const dim3 grid = grid_of(gemv_blocks + qblocks);
     const uint32_t rbl = gemv_xcd_split(n_expert, (n_tok + tg - 1u) / tg, tg);
     if (tg == 1u)
         hipLaunchKernelGGL(router_logits_q8_kernel<1>, grid, dim3(256), 0, pk::stream(), (float *)logits,

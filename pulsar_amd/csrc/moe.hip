@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256) void slot_sum_kernel(float *__restrict__ out,
                                                        const float *__restrict__ partial,
                                                        uint32_t out_dim, uint32_t n_used,
                                                        uint64_t total) {
-    const uint64_t gid = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const uint64_t gid = (uint64_t)block_index() * blockDim.x + threadIdx.x;
     if (gid >= total) return;
     const uint64_t token = gid / out_dim;
     const uint64_t row = gid - token * out_dim;
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(256) void slot_sum_bias_kernel(float *__restrict__ 
                                                             const pulsar_expert_ptrs *__restrict__ ptrs,
                                                             const float *__restrict__ weights,
                                                             uint32_t out_dim, uint32_t n_used, uint64_t total) {
-    const uint64_t gid = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const uint64_t gid = (uint64_t)block_index() * blockDim.x + threadIdx.x;
     if (gid >= total) return;
     const uint64_t token = gid / out_dim;
     const uint64_t row = gid - token * out_dim;
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(256) void down_bias_kernel(float *__restrict__ out,
                                                         const float *__restrict__ weights,
                                                         uint32_t out_dim, uint32_t n_used,
                                                         uint64_t total) {
-    const uint64_t gid = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const uint64_t gid = (uint64_t)block_index() * blockDim.x + threadIdx.x;
     if (gid >= total) return;
     const uint64_t token = gid / out_dim;
     const uint64_t row = gid - token * out_dim;
@@ -845,8 +845,9 @@ extern "C" int pulsar_moe_down_experts(void *partial, const void *selected, cons
 extern "C" int pulsar_moe_slot_sum(void *out, const void *partial, uint32_t out_dim, uint32_t n_used,
                                    uint32_t n_tok) {
     if (!out || !partial || out_dim == 0 || n_used == 0 || n_tok == 0) return reject("moe slot sum");
-    const uint64_t total = (uint64_t)n_tok * out_dim;
-    hipLaunchKernelGGL(slot_sum_kernel, dim3((uint32_t)((total + 255u) / 256u)), dim3(256), 0, pk::stream(),
+    const uint64_t total = (uint64_t)n_tok * out_dim, blocks = (total + 255u) / 256u;
+    if (blocks >> 31) return reject("moe slot sum (size)");
+    hipLaunchKernelGGL(slot_sum_kernel, grid_of(blocks), dim3(256), 0, pk::stream(),
                        (float *)out, (const float *)partial, out_dim, n_used, total);
     return launch_ok("moe slot sum launch");
 }
@@ -855,8 +856,9 @@ extern "C" int pulsar_moe_down_bias(void *out, const void *ptrs, const void *wei
                                     uint32_t out_dim, uint32_t n_used, uint32_t n_tok) {
     if (!out || !ptrs || !weights || out_dim == 0 || n_used == 0 || n_tok == 0)
         return reject("moe down bias");
-    const uint64_t total = (uint64_t)n_tok * out_dim;
-    hipLaunchKernelGGL(down_bias_kernel, dim3((uint32_t)((total + 255u) / 256u)), dim3(256), 0, pk::stream(),
+    const uint64_t total = (uint64_t)n_tok * out_dim, blocks = (total + 255u) / 256u;
+    if (blocks >> 31) return reject("moe down bias (size)");
+    hipLaunchKernelGGL(down_bias_kernel, grid_of(blocks), dim3(256), 0, pk::stream(),
                        (float *)out, (const pulsar_expert_ptrs *)ptrs, (const float *)weights,
                        out_dim, n_used, total);
     return launch_ok("moe down bias launch");
@@ -866,8 +868,9 @@ extern "C" int pulsar_moe_slot_sum_bias(void *out, const void *partial, const vo
                                         uint32_t out_dim, uint32_t n_used, uint32_t n_tok) {
     if (!out || !partial || !ptrs || !weights || out_dim == 0 || n_used == 0 || n_tok == 0)
         return reject("moe slot sum bias");
-    const uint64_t total = (uint64_t)n_tok * out_dim;
-    hipLaunchKernelGGL(slot_sum_bias_kernel, dim3((uint32_t)((total + 255u) / 256u)), dim3(256), 0, pk::stream(),
+    const uint64_t total = (uint64_t)n_tok * out_dim, blocks = (total + 255u) / 256u;
+    if (blocks >> 31) return reject("moe slot sum bias (size)");
+    hipLaunchKernelGGL(slot_sum_bias_kernel, grid_of(blocks), dim3(256), 0, pk::stream(),
                        (float *)out, (const float *)partial, (const pulsar_expert_ptrs *)ptrs, (const float *)weights,
                        out_dim, n_used, total);
     return launch_ok("moe slot sum bias launch");

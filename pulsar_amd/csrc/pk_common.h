@@ -38,6 +38,8 @@ static inline dim3 grid_of(uint64_t n, uint32_t unit = 1) {
     return dim3((uint32_t)x, (uint32_t)y);
 }
 PK_DEV uint32_t block_index() { return blockIdx.y * gridDim.x + blockIdx.x; }
+// Values of an f32 row at most: a block of 256 past it still has 32-bit indices
+constexpr uint32_t kMaxRow = 0xffffff00u;
 
 static inline int reject(const char *what) {
     fprintf(stderr, "pulsar-kernels: %s: invalid arguments\n", what);

@@ -16,7 +16,7 @@ __global__ __launch_bounds__(256) void quantize_q8k_kernel(pulsar_block_q8_K *__
                                                            const float *__restrict__ x,
                                                            uint32_t in_dim, uint32_t nb,
                                                            uint64_t n_blocks) {
-    const uint64_t gblk = (uint64_t)blockIdx.x * (blockDim.x / 64u) + threadIdx.x / 64u;
+    const uint64_t gblk = (uint64_t)block_index() * (blockDim.x / 64u) + threadIdx.x / 64u;
     if (gblk >= n_blocks) return;  // whole wave
     const uint64_t row = gblk / nb;
     const uint32_t b = (uint32_t)(gblk - row * nb);
@@ -41,12 +41,12 @@ __global__ __launch_bounds__(256) void bw_read_kernel(const u32x4 *__restrict__ 
 }  // namespace pk
 
 extern "C" int pulsar_quantize_q8_K(void *out, const void *x, uint32_t in_dim, uint32_t n_rows) {
-    if (!out || !x || in_dim == 0 || n_rows == 0) return pk::reject("q8_K quantize");
+    if (!out || !x || in_dim == 0 || in_dim > pk::kMaxRow || n_rows == 0) return pk::reject("q8_K quantize");
     const uint32_t nb = (in_dim + 255u) / 256u;
     const uint64_t n_blocks = (uint64_t)nb * n_rows;
     const uint64_t grid = (n_blocks + 3u) / 4u;
     if (grid > 0x7fffffffull) return pk::reject("q8_K quantize");
-    hipLaunchKernelGGL(pk::quantize_q8k_kernel, dim3((uint32_t)grid), dim3(256), 0, pk::stream(),
+    hipLaunchKernelGGL(pk::quantize_q8k_kernel, pk::grid_of(grid), dim3(256), 0, pk::stream(),
                        (pulsar_block_q8_K *)out, (const float *)x, in_dim, nb, n_blocks);
     return pk::launch_ok("q8_K quantize launch");
 }

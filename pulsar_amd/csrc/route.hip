@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void route_ptrs_kernel(pulsar_expert_ptrs *__r
                                                          SharedSlots shared, uint32_t n_shared,
                                                          uint32_t n_tok, uint32_t k_used) {
     const uint32_t n_slots = k_used + n_shared;
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const uint64_t i = (uint64_t)block_index() * blockDim.x + threadIdx.x;
     if (i >= (uint64_t)n_tok * n_slots) return;
     const uint32_t t = (uint32_t)(i / n_slots), s = (uint32_t)(i % n_slots);
     pulsar_expert_ptrs p;
@@ -447,8 +447,9 @@ extern "C" int pulsar_moe_route_ptrs(void *ptrs, void *slot_weights, const void 
         return pk::reject("moe route ptrs");
     pk::SharedSlots sh = {};
     for (uint32_t i = 0; i < n_shared; i++) sh.p[i] = shared[i];
-    const uint64_t total = (uint64_t)n_tok * (k_used + n_shared);
-    hipLaunchKernelGGL(pk::route_ptrs_kernel, dim3((uint32_t)((total + 255u) / 256u)), dim3(256), 0, pk::stream(),
+    const uint64_t blocks = ((uint64_t)n_tok * ((uint64_t)k_used + n_shared) + 255u) / 256u;
+    if (blocks >> 31) return pk::reject("moe route ptrs (size)");
+    hipLaunchKernelGGL(pk::route_ptrs_kernel, pk::grid_of(blocks), dim3(256), 0, pk::stream(),
                        (pulsar_expert_ptrs *)ptrs, (float *)slot_weights, (const int32_t *)selected,
                        (const float *)router_weights, *bank, n_expert, sh, n_shared, n_tok, k_used);
     return pk::launch_ok("moe route ptrs launch");

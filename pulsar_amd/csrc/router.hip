@@ -12,15 +12,16 @@ template <uint32_t TG>
 __global__ __launch_bounds__(256) void matmul_f32_kernel(float *__restrict__ out, const float *__restrict__ w,
                                                          const float *__restrict__ x, uint32_t in_dim,
                                                          uint32_t out_dim, uint32_t n_tok, uint32_t rb_log2) {
-    gemv_block<TG>(out, w, x, nullptr, in_dim, out_dim, n_tok,
-                   gemv_item(blockIdx.x, out_dim, gridDim.x / out_dim, rb_log2));
+    const uint32_t block = block_index(), n_grp = (n_tok + TG - 1u) / TG;
+    if (block >= out_dim * n_grp) return;  // block-uniform
+    gemv_block<TG>(out, w, x, nullptr, in_dim, out_dim, n_tok, gemv_item(block, out_dim, n_grp, rb_log2));
 }
 
 // x[r][i] += bias[i] (pulsar_kernels.cu:3621-3629)
 __global__ __launch_bounds__(256) void add_bias_rows_kernel(float *__restrict__ x,
                                                             const float *__restrict__ bias,
                                                             uint32_t dim, uint64_t total) {
-    const uint64_t gid = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const uint64_t gid = (uint64_t)block_index() * blockDim.x + threadIdx.x;
     if (gid >= total) return;
     x[gid] += bias[gid % dim];
 }
@@ -39,11 +40,12 @@ __global__ __launch_bounds__(64) void router_select_kernel(int32_t *__restrict__
                                                            const float *__restrict__ bias,
                                                            uint32_t n_expert, uint32_t k_used,
                                                            float weight_scale, uint32_t mode,
-                                                           uint32_t n_shexp) {
+                                                           uint32_t n_shexp, uint32_t n_tok) {
     __shared__ int32_t sel_l[64u * kMaxPerLane + 64u];
     __shared__ float w_l[64u * kMaxPerLane + 64u];
     __shared__ float es_l;
-    const uint32_t token = blockIdx.x;
+    const uint32_t token = block_index();
+    if (token >= n_tok) return;  // block-uniform
     const uint32_t lane = threadIdx.x;
     const uint32_t sink = mode == 2u ? n_shexp : 0u;
     const uint32_t n_logit = n_expert + sink;
@@ -105,13 +107,14 @@ __global__ __launch_bounds__(64) void router_select_kernel(int32_t *__restrict__
 
 extern "C" int pulsar_matmul_f32(void *out, const void *w, const void *x, uint32_t in_dim,
                                  uint32_t out_dim, uint32_t n_tok) {
-    if (!out || !w || !x || in_dim == 0 || out_dim == 0 || n_tok == 0) return pk::reject("matmul f32");
+    if (!out || !w || !x || in_dim == 0 || in_dim > pk::kMaxRow || out_dim == 0 || n_tok == 0)
+        return pk::reject("matmul f32");
     // tokens in pairs (1 for a single token); one block per (row, pair): c4
     // layer 138.8 -> 137.5 us against groups of 4 (the same sums), 8 slower
     const uint32_t tg = n_tok == 1u ? 1u : 2u;
-    const uint64_t work = (uint64_t)out_dim * ((n_tok + tg - 1u) / tg);
-    if (work > 0x7fffffffull) return pk::reject("matmul f32 (size)");
-    const dim3 grid((uint32_t)work);
+    const uint64_t work = (uint64_t)out_dim * (((uint64_t)n_tok + tg - 1u) / tg);
+    if (work >> 31) return pk::reject("matmul f32 (size)");
+    const dim3 grid = pk::grid_of(work);
     const uint32_t rbl = pk::gemv_xcd_split(out_dim, (n_tok + tg - 1u) / tg, tg);
     if (tg == 1u)
         hipLaunchKernelGGL(pk::matmul_f32_kernel<1>, grid, dim3(256), 0, pk::stream(), (float *)out,
@@ -124,9 +127,10 @@ extern "C" int pulsar_matmul_f32(void *out, const void *w, const void *x, uint32
 
 extern "C" int pulsar_add_bias_rows(void *x, const void *bias, uint32_t dim, uint32_t rows) {
     if (!x || !bias || dim == 0 || rows == 0) return pk::reject("add bias rows");
-    const uint64_t total = (uint64_t)rows * dim;
-    hipLaunchKernelGGL(pk::add_bias_rows_kernel, dim3((uint32_t)((total + 255u) / 256u)), dim3(256),
-                       0, pk::stream(), (float *)x, (const float *)bias, dim, total);
+    const uint64_t total = (uint64_t)rows * dim, blocks = (total + 255u) / 256u;
+    if (blocks >> 31) return pk::reject("add bias rows (size)");
+    hipLaunchKernelGGL(pk::add_bias_rows_kernel, pk::grid_of(blocks), dim3(256), 0, pk::stream(), (float *)x,
+                       (const float *)bias, dim, total);
     return pk::launch_ok("add bias rows launch");
 }
 
@@ -136,13 +140,13 @@ extern "C" int pulsar_router_select(void *selected, void *weights, const void *l
                                     float weight_scale, uint32_t n_tok, uint32_t softmax_mode,
                                     uint32_t n_shexp) {
     if (!selected || !weights || !logits || n_expert == 0 || k_used == 0 || k_used > n_expert ||
-        n_tok == 0 || softmax_mode > 2u || (softmax_mode != 2u && n_shexp != 0) ||
+        n_tok == 0 || n_tok > 0x7fffffffu || softmax_mode > 2u || (softmax_mode != 2u && n_shexp != 0) ||
         n_expert + (softmax_mode == 2u ? n_shexp : 0u) > 1024u || n_expert > 64u * pk::kMaxPerLane)
         return pk::reject("router select");
 #define PK_SELECT(J)                                                                                        \
-    hipLaunchKernelGGL(pk::router_select_kernel<J>, dim3(n_tok), dim3(64), 0, pk::stream(), (int32_t *)selected, \
+    hipLaunchKernelGGL(pk::router_select_kernel<J>, pk::grid_of(n_tok), dim3(64), 0, pk::stream(), (int32_t *)selected, \
                        (float *)weights, (const float *)logits, (const float *)bias, n_expert, k_used,           \
-                       weight_scale, softmax_mode, n_shexp)
+                       weight_scale, softmax_mode, n_shexp, n_tok)
     // the fewest experts per lane that hold them all (a lane's best is a
     // scan over its J entries in every round)
     if (n_expert <= 64u)
