@@ -15,6 +15,12 @@
  *     (crates/kernels/build.rs:42-48), so a thread-local graph capture begun
  *     on it records them; pulsar_set_stream selects another stream. Nothing
  *     here synchronises.
+ *   - one axis of a launch holds fewer than 2^32 threads, and the runtime leaves
+ *     out what is past them without an error: calls that go by values or rows
+ *     take two axes (up to 2^31 - 1 blocks: of 256 values, of 4 q8_K blocks, of
+ *     an f32 product's row and two tokens, of a routed token), the MoE stages
+ *     refuse the rows of an expert that one does not hold (fewer than 2^24 always
+ *     go). f32 rows have at most 2^32 - 256 values.
  *
  * Byte layouts are the GGUF/ggml ones (crates/gguf/src/lib.rs:145-180):
  *   Q2_K 84 B / 256, Q4_K 144 B / 256, Q6_K 210 B / 256, IQ2_XXS 66 B / 256,

@@ -292,6 +292,7 @@ struct PairRoutedLaunch {
     int go_j() {
         const uint32_t rpb = kRoutedWaves<Q> * (64u >> g.l2);
         const dim3 grid((mid_dim + rpb - 1u) / rpb, n_slots, n_tok);
+        if (!axis_fits(grid, 64u * kRoutedWaves<Q>)) return reject("moe pair routed (size)");
         hipLaunchKernelGGL((moe_pair_routed_kernel<Q, U, J, NPL, 1>), grid, dim3(64u * kRoutedWaves<Q>), 0, pk::stream(),
                            (float *)mid, (pulsar_expert_ptrs *)ptrs_out, (float *)slot_w_out, (int32_t *)sel_out,
                            (float *)w_out, (const float *)logits, (const float *)rbias, n_expert, k_used, scale,
@@ -328,6 +329,7 @@ struct DownF32Launch {
         const size_t lds = (size_t)n_used * g.blocks * kActLdsPitch + (size_t)n_pass * n_used * 16u * 4u;
         uint32_t nw = n_pass * n_used;  // one (pass, slot) dot per wave where it fits
         nw = nw < 4u ? 4u : nw > kFusedDownWaves ? kFusedDownWaves : nw;
+        if (!axis_fits(grid, 64u * nw)) return reject("moe down f32 (size)");
         hipLaunchKernelGGL((moe_down_f32_kernel<Q, U, NPL>), grid, dim3(64u * nw), lds, pk::stream(), (float *)out,
                            (const pulsar_expert_ptrs *)ptrs, (const float *)slot_w, (const float *)mid, g.n_units,
                            g.nblk32, g.l2, g.blocks, mid_dim, out_dim, n_used, row_bytes, add_bias, n_pass);

@@ -221,6 +221,7 @@ static int dispatch_matvec(float *out, const uint8_t *w, const pulsar_block_q8_K
     } else {
         // wider rows: one wave per row, streamed in 16-super-block slices
         const dim3 grid((out_dim + 3u) / 4u, n_tok <= 1u ? 1u : (n_tok + 3u) / 4u);
+        if (!axis_fits(grid, 256u)) return reject("matmul_kq (size)");
         if (n_tok == 1u)
             hipLaunchKernelGGL((matvec_wide_kernel<Q, 1, E>), grid, dim3(256), 0, pk::stream(), out, w, xq, n_units,
                                nblk32, in_blocks, out_dim, n_tok, row_bytes, epi);

@@ -550,7 +550,7 @@ template <typename E>
 int launch_gemm(uint32_t quant, float *out, const uint8_t *w, const pulsar_block_q8_K *xq, uint32_t in_dim,
                 uint32_t out_dim, uint32_t n_tok, uint64_t row_bytes, const E &epi) {
     const uint32_t nb = in_dim / 256u;
-    if ((uint64_t)((out_dim + 31u) / 32u) > 65535u) return -1;  // grid y
+    if ((uint64_t)((out_dim + 31u) / 32u) > 65535u || n_tok >> 29) return -1;  // grid y; the threads of x, 8 a token
     switch (quant) {
     case PULSAR_QUANT_Q6_K: return launch_gemm_q<PULSAR_QUANT_Q6_K>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi);
     case PULSAR_QUANT_Q4_K: return launch_gemm_q<PULSAR_QUANT_Q4_K>(out, w, xq, nb, out_dim, n_tok, row_bytes, epi);
@@ -1395,10 +1395,13 @@ int launch_grouped_mmq_kq(bool pair, uint32_t quant, float *out, const G &src, c
     const uint32_t lst_off = (pmax * per_pair + 15u) & ~15u;
     const size_t lds = (size_t)lst_off + lst_bytes;
 #define PK_GQ(Q, P)                                                                                              \
-    hipLaunchKernelGGL((moe_grouped_mmq_kq_kernel<Q, P, G>),                                                     \
-                       dim3((n_rows + kGqBlockRows<Q, P> - 1u) / kGqBlockRows<Q, P>, n_group),                     \
-                       dim3(64u * kGqWaves<Q>), lds, pk::stream(), out, src, weights, act, k_blocks, lim, n_rows, \
-                       n_used, row_bytes, act_op, pmax, lst_off)
+    do {                                                                                                         \
+        const dim3 grid((n_rows + kGqBlockRows<Q, P> - 1u) / kGqBlockRows<Q, P>, n_group);                       \
+        if (!axis_fits(grid, 64u * kGqWaves<Q>)) return reject("moe grouped (size)");                            \
+        hipLaunchKernelGGL((moe_grouped_mmq_kq_kernel<Q, P, G>), grid, dim3(64u * kGqWaves<Q>), lds,             \
+                           pk::stream(), out, src, weights, act, k_blocks, lim, n_rows, n_used, row_bytes,       \
+                           act_op, pmax, lst_off);                                                               \
+    } while (0)
     if (quant == PULSAR_QUANT_Q2_K && pair)
         PK_GQ(PULSAR_QUANT_Q2_K, true);
     else if (quant == PULSAR_QUANT_Q2_K)

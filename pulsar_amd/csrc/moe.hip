@@ -465,6 +465,7 @@ struct PairLaunch {
         const bool two = (uint64_t)((mid_dim + rpb - 1u) / rpb) * n_used * n_tok > kPairOneRoundBlocks;
         const uint32_t rpw = two ? 2u : 1u;
         const dim3 grid((mid_dim + rpw * rpb - 1u) / (rpw * rpb), n_used, n_tok);
+        if (!axis_fits(grid, 256u)) return reject("moe pair swiglu (size)");
 #define PK_PAIR_GO(R)                                                                                          \
     hipLaunchKernelGGL((moe_pair_kernel<Q, U, NPL, R>), grid, dim3(256), 0, pk::stream(), (float *)mid,       \
                        (const pulsar_expert_ptrs *)ptrs, (const float *)weights, (const pulsar_block_q8_K *)xq, \
@@ -493,6 +494,7 @@ struct DownLaunch {
     int go() {
         const uint32_t rpp = 64u >> g.l2;
         const dim3 grid((out_dim + rpp - 1u) / rpp, n_tok);
+        if (!axis_fits(grid, 256u)) return reject("moe down (size)");
         if (weights)
             hipLaunchKernelGGL((moe_down_kernel<Q, U, NPL, true>), grid, dim3(256), 0, pk::stream(), (float *)out,
                                (const pulsar_expert_ptrs *)ptrs, (const pulsar_block_q8_K *)midq, g.n_units,
@@ -518,6 +520,7 @@ struct PairGroupedLaunch {
     int run() {
         const uint32_t rpb = kWaves * PK_GRP_PPW * (64u >> g.l2);
         const dim3 grid((mid_dim + rpb - 1u) / rpb, n_group);
+        if (!axis_fits(grid, 256u)) return reject("moe pair swiglu grouped (size)");
         const uint32_t pmax = grouped_pmax(g.blocks);
         const uint32_t lst_off = pmax * g.blocks * kActLdsPitch;
         hipLaunchKernelGGL((moe_pair_grouped_kernel<Q, U, G>), grid, dim3(256), lst_off + lst_bytes, pk::stream(),
@@ -540,6 +543,7 @@ struct DownGroupedLaunch {
     int run() {
         const uint32_t rpb = kWaves * PK_GRP_PPW * (64u >> g.l2);
         const dim3 grid((out_dim + rpb - 1u) / rpb, n_group);
+        if (!axis_fits(grid, 256u)) return reject("moe down grouped (size)");
         const uint32_t pmax = grouped_pmax(g.blocks);
         const uint32_t lst_off = pmax * g.blocks * kActLdsPitch;
         hipLaunchKernelGGL((moe_down_grouped_kernel<Q, U, G>), grid, dim3(256), lst_off + lst_bytes, pk::stream(),

@@ -37,6 +37,8 @@ static inline dim3 grid_of(uint64_t n, uint32_t unit = 1) {
     const uint64_t y = (n + (1u << 21) - 1u) >> 21, x = ((n + y - 1u) / y + unit - 1u) / unit * unit;
     return dim3((uint32_t)x, (uint32_t)y);
 }
+// Whether the first axis of a grid holds its blocks of so many threads
+static inline bool axis_fits(const dim3 &grid, uint32_t threads) { return (uint64_t)grid.x * threads < 1ull << 32; }
 PK_DEV uint32_t block_index() { return blockIdx.y * gridDim.x + blockIdx.x; }
 // Values of an f32 row at most: a block of 256 past it still has 32-bit indices
 constexpr uint32_t kMaxRow = 0xffffff00u;

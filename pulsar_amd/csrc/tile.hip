@@ -126,7 +126,7 @@ static int launch_tile_gemm_q(float *out, const uint8_t *w, const pulsar_block_q
 #define PK_TILE(WR, WK, NS)                                                                                        \
     do {                                                                                                           \
         const uint64_t n_item = tile_items<Q, WR, WK, NS>(out_dim, n_tok);                                         \
-        if (n_item > 0x7ffffff0ull) return -1;                                                                     \
+        if (n_item > 0xfffff0ull) return -1;                                                                       \
         hipLaunchKernelGGL((tile_gemm_kernel<Q, WR, WK, NS, E>), dim3((uint32_t)((n_item + 7u) & ~7ull)), dim3(256), 0, \
                            pk::stream(), out, w, xq, nb, out_dim, n_tok, row_bytes,                                 \
                            (n_tok + 16u * NS - 1u) / (16u * NS), (uint32_t)n_item, epi);                            \

@@ -248,10 +248,12 @@ int launch_tile_experts(bool pair, uint32_t quant, float *out, const ExpertGroup
                         const pulsar_block_q8_K *act, uint32_t k_dim, uint32_t n_rows, uint32_t n_used,
                         uint32_t n_group, uint64_t row_bytes, uint32_t act_op, uint32_t lst_bytes, bool shared_only) {
 #define PK_LAUNCH(Q, P)                                                                                               \
-    hipLaunchKernelGGL((tile_experts_kernel<Q, P, 4>),                                                                \
-                       dim3((n_rows + GroupTile<Q, P, 4>::kRows - 1u) / GroupTile<Q, P, 4>::kRows, n_group), dim3(256), \
-                       lst_bytes, pk::stream(), out, src, weights, act, k_dim / 256u, n_rows, n_used, row_bytes,      \
-                       act_op, (uint32_t)shared_only)
+    do {                                                                                                              \
+        const dim3 grid((n_rows + GroupTile<Q, P, 4>::kRows - 1u) / GroupTile<Q, P, 4>::kRows, n_group);              \
+        if (!axis_fits(grid, 256u)) return reject("moe experts (size)");                                              \
+        hipLaunchKernelGGL((tile_experts_kernel<Q, P, 4>), grid, dim3(256), lst_bytes, pk::stream(), out, src,        \
+                           weights, act, k_dim / 256u, n_rows, n_used, row_bytes, act_op, (uint32_t)shared_only);     \
+    } while (0)
 #define PK_CASE(Q)                  \
     case Q:                         \
         if (pair)                   \

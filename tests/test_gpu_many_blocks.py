@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from pulsar_amd import kernels as K
+from pulsar_amd import synth
+from pulsar_amd.formats import QUANT_IQ4_NL, QUANT_NVFP4, QUANT_Q4_K, row_bytes
 from tests.gpu_util import up_f32, zeros_f32
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +109,22 @@ def test_router_select(dev):
     torch.cuda.synchronize()
     assert torch.equal(selected[:, 0], (logits[:, 1] > logits[:, 0]).int())  # the first of equal ones
     assert (weights == 2.5).all()  # a softmax over one winner
+
+
+@pytest.mark.parametrize("quant,n_tok", [(QUANT_IQ4_NL, 300_001), (QUANT_NVFP4, 2_200_001), (QUANT_Q4_K, 2_200_001)])
+def test_products_of_many_tokens(dev, quant, n_tok):
+    """More token groups than 2^16: the tokens repeat, so do the rows of the product."""
+    rows, cols, period = 16, 256, 1000
+    w = torch.from_numpy(synth.quant_matrix(quant, rows, cols, np.random.default_rng(1)).view(np.uint8).reshape(-1)).to(dev)
+    x = small((period, cols), 1, dev)
+    xq = torch.zeros((period, 292), dtype=torch.uint8, device=dev)
+    K.quantize_q8_k(xq, x, cols, period)
+    torch.cuda.synchronize()
+    many = xq.repeat(-(-n_tok // period), 1)[:n_tok].contiguous()
+    out = torch.full((n_tok, rows), 1e30, device=dev)
+    torch.cuda.synchronize()
+    K.matmul_kq(out, w, many, cols, rows, n_tok, row_bytes(quant, cols), quant)
+    torch.cuda.synchronize()
+    assert (out[:period].abs() < 1e6).all()
+    whole = n_tok // period * period
+    assert (out[:whole].view(-1, period, rows) == out[:period]).all() and torch.equal(out[whole:], out[:n_tok - whole])
