@@ -259,9 +259,11 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs<TYPE> a) {
 // 1 / (1 + e^-z) in 64 bits, within some units in the last place. With E = e^-|z| in
 // (0, 1] it is E^(z < 0) / (1 + E), where nothing overflows. e^-|z| = 2^n e^r, r within
 // ln 2 / 2 (ln 2 in two parts), by the series to r^12 (what is left: 2^-52); the
-// reciprocal of 1 .. 2 from the instruction's 2^-24 in two Newton steps.
+// reciprocal of 1 .. 2 from the instruction's 2^-24 in two Newton steps. Of z < 0 it is
+// 2^LIFT times as large.
+template <int32_t LIFT = 0>
 PK_DEV double sigmoid64(double z) {
-    const double x = __builtin_fmax(-__builtin_fabs(z), -800.0);  // E is 0 from -745 on
+    const double x = __builtin_fmax(-__builtin_fabs(z), -800.0 - 2 * LIFT);  // E is 0 from -745 - 0.7 LIFT on
     const double n = __builtin_rint(x * 1.4426950408889634);
     double r = __builtin_fma(n, -0.6931471805599453, x);  // ln 2 rounded, and what is left of it
     r = __builtin_fma(n, -2.3190468138462996e-17, r);
@@ -270,22 +272,22 @@ PK_DEV double sigmoid64(double z) {
                             1.0 / 120.0,      1.0 / 24.0,      1.0 / 6.0,      0.5,           1.0,          1.0};
 #pragma unroll
     for (int k = 0; k < 12; k++) e = __builtin_fma(e, r, c[k]);
-    e = __builtin_ldexp(e, (int)n);
-    const double d = 1.0 + e;
+    const double d = 1.0 + __builtin_ldexp(e, (int)n);
     double y = __builtin_amdgcn_rcp(d);
     y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
     y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
-    return (z < 0.0 ? e : 1.0) * y;
+    return (z < 0.0 ? __builtin_ldexp(e, (int)n + LIFT) : 1.0) * y;
 }
-// The gated combine of pk::glu in 64 bits
+// The gated combine of pk::glu in 64 bits; 2^LIFT times it where the gate is below 0
+template <int32_t LIFT = 0>
 PK_DEV double glu64(float g, float u, uint32_t op) {
     double v = g, w = u;
     if (op == PULSAR_ACT_SWIGLU_OAI) {
         v = v > 7.0 ? 7.0 : v;  // NaN stays
         w = (w > 7.0 ? 7.0 : w < -7.0 ? -7.0 : w) + 1.0;
-        return v * sigmoid64(1.702 * v) * w;
+        return v * sigmoid64<LIFT>(1.702 * v) * w;
     }
-    return v * sigmoid64(v) * w;
+    return v * sigmoid64<LIFT>(v) * w;
 }
 
 template <uint32_t TYPE>
@@ -298,21 +300,25 @@ struct QuantArgs {
     uint32_t dim, n_rows, act_op;
 };
 
-template <uint32_t TYPE, uint32_t V>
+template <int32_t LIFT, uint32_t TYPE, uint32_t V>
 PK_DEV void quant_values(const QuantArgs<TYPE> &a, uint64_t row, uint32_t c0, uint32_t n, double (&v)[V]) {
     float g[V], u[V];
     load_row<TYPE>(a.x + row * a.x_stride + c0, n, g);
     if (a.up) {
         load_row<TYPE>(a.up + row * a.up_stride + c0, n, u);
 #pragma unroll
-        for (uint32_t k = 0; k < V; k++) v[k] = glu64(g[k], u[k], a.act_op);
+        for (uint32_t k = 0; k < V; k++) v[k] = glu64<LIFT>(g[k], u[k], a.act_op);
     } else {
 #pragma unroll
         for (uint32_t k = 0; k < V; k++) v[k] = g[k];
     }
 }
-// A row of any length and values, read twice and combined in 64 bits
-template <uint32_t TYPE>
+// A row of any length and values, read twice and combined in 64 bits. Where E leaves the
+// normal numbers, gates below -708, values are below 2^-884 (E 2^-1022, the gate 2^10, up
+// 2^128) and short of bits, and 127 / A overflows for A < 2^-1017. So a row whose largest
+// is below 2^-800 is looked at again with 2^600 times its values: they have all their bits
+// then. Its gates that are not below 0 have values of 0 (others are above 2^-300).
+template <int32_t LIFT = 0, uint32_t TYPE>
 PK_DEV void quantize_row(const QuantArgs<TYPE> &a, RowStats &lds) {
     constexpr uint32_t V = kLane<TYPE>;
     const uint32_t step = V * blockDim.x;
@@ -320,21 +326,28 @@ PK_DEV void quantize_row(const QuantArgs<TYPE> &a, RowStats &lds) {
     double v[V], none = 0.0;
     uint64_t top = 0u;
     for (uint32_t c0 = V * threadIdx.x; c0 < a.dim; c0 += step) {
-        quant_values(a, row, c0, inside<V>(c0, a.dim), v);
+        quant_values<LIFT>(a, row, c0, inside<V>(c0, a.dim), v);
 #pragma unroll
         for (uint32_t k = 0; k < V; k++) top = max_bits(top, size_bits(v[k]));
     }
     top = group_max64<64>(top);
     block_stats(lds, none, top);
     const double largest = __builtin_bit_cast(double, top), factor = code_factor(largest);
+    if constexpr (LIFT == 0) {
+        if (largest > 0.0 && largest < 0x1p-800) {  // block-uniform
+            __syncthreads();  // lds is read
+            quantize_row<600>(a, lds);
+            return;
+        }
+    }
     for (uint32_t c0 = V * threadIdx.x; c0 < a.dim; c0 += step) {
         const uint32_t n = inside<V>(c0, a.dim);
-        quant_values(a, row, c0, n, v);
+        quant_values<LIFT>(a, row, c0, n, v);
         int8_t q[V];
         codes_of(v, factor, q);
         store_row((int8_t *)a.q + row * a.q_stride + c0, n, q);
     }
-    if (threadIdx.x == 0u) a.scales[row] = (float)(largest * (1.0 / 127.0));
+    if (threadIdx.x == 0u) a.scales[row] = LIFT ? 0.0f : (float)(largest * (1.0 / 127.0));
 }
 template <uint32_t TYPE>
 __global__ __launch_bounds__(1024) void quantize_i8_long_kernel(QuantArgs<TYPE> a) {
