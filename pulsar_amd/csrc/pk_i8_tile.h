@@ -429,8 +429,7 @@ static uint64_t i8_items(const I8Args &a) {
 }
 template <uint32_t TYPE, typename T>
 static int launch_i8_tile(const I8Args &a) {
-    const uint64_t n = i8_items<T>(a);
-    if (n >> 31) return reject("matmul_i8 (size)");
+    const uint64_t n = i8_items<T>(a);  // below 2^31: the entry point refuses more
     hipLaunchKernelGGL((i8_tile_kernel<TYPE, T>), grid_of(n, 8u), dim3(T::kThreads), 0, pk::stream(), a,
                        (a.n_tok + T::BM - 1u) / T::BM, (a.out_dim + T::BN - 1u) / T::BN, (uint32_t)n);
     return launch_ok("matmul_i8 tile launch");

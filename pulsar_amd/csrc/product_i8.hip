@@ -25,6 +25,9 @@ extern "C" int pulsar_matmul_i8(void *out, const void *w, const void *w_scales, 
         overlap(out, on, w, (u128)(out_dim - 1u) * w_stride + in_dim) || overlap(out, on, w_scales, 4 * (u128)out_dim) ||
         overlap(out, on, x_scales, 4 * (u128)n_tok) || (bias && overlap(out, on, bias, 4 * (u128)out_dim)))
         return reject("matmul_i8 (overlap)");
+    // no tile that a product takes counts more than these: finer ones are for up to 64 tokens
+    // or 256 tiles
+    if ((((uint64_t)n_tok + 127u) / 128u * (((uint64_t)out_dim + 127u) / 128u)) >> 31) return reject("matmul_i8 (size)");
     const I8Args a = {(const uint8_t *)w, (const uint8_t *)x, (const float *)w_scales, (const float *)x_scales,
                       (const float *)bias, residual, out, w_stride, x_stride, out_stride, res_stride, in_dim, out_dim,
                       n_tok, act};

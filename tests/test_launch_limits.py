@@ -5,8 +5,9 @@ import pytest
 import torch
 
 from pulsar_amd import kernels as K
-from pulsar_amd.formats import ACT_SILU, QUANT_IQ4_XS, QUANT_MXFP4, QUANT_Q2_K, QUANT_Q3_K, QUANT_Q4_K, row_bytes
-from tests.test_int8_arguments import A, lib, said  # noqa: F401
+from pulsar_amd.formats import (ACT_SILU, QUANT_IQ4_XS, QUANT_MXFP4, QUANT_Q2_K, QUANT_Q3_K, QUANT_Q4_K, TYPE_BF16, TYPE_F16,
+                                TYPE_F32, row_bytes)
+from tests.test_int8_arguments import A, lib, product, said  # noqa: F401
 from tests.test_operator_refusals import bank
 
 COLS = 4096  # a row is a wave's
@@ -83,3 +84,16 @@ def test_the_most_rows_reach_a_launch(capfd, call, rows):
     lambda: K.moe_route_ptrs(A[0], A[1], A[2], A[3], bank(), 32, [], 2**31, 2**8)])
 def test_sizes_past_two_axes(capfd, call):
     assert said(capfd, call)
+
+
+@pytest.mark.parametrize("in_dim", [300, 304])  # rows that are not on 16 bytes, and that are
+@pytest.mark.parametrize("kind", [TYPE_F32, TYPE_F16, TYPE_BF16])
+def test_int8_product_refuses_2_31_tiles(capfd, in_dim, kind):
+    """Of 128 tokens x 128 channels, whatever tile the product would take."""
+    call = lambda T, n: product(out=1 << 61, residual=0, in_dim=in_dim, out_dim=n, n_tok=T, type=kind)  # noqa: E731
+    for T, n in ((128 * 127 + 1, 2**31 - 1), (2**31 - 1, 128 * 127 + 1), (128 * 2**15 + 1, 128 * (2**16 - 1))):
+        assert "matmul_i8 (size)" in said(capfd, lambda: call(T, n))
+    if torch.cuda.is_available():
+        return  # these addresses are nobody's
+    for T, n in ((128 * 127, 2**31 - 1), (2**31 - 1, 128 * 127), (128 * 2**15, 128 * (2**16 - 1)), (2, 2**31 - 1)):
+        assert not said(capfd, lambda: call(T, n))
