@@ -8,9 +8,11 @@
 // divides every value of the row alike, so codes and the largest size are those of s *
 // gain, known without it. Sums, products and codes in 64 bits cost about what the bytes
 // do: a value of a norm is 7 to 17 bytes of traffic and 35 instructions, most of them at the
-// rate of f32's. Measured (GB/s of what has to move): norm of 8192 rows of 4096 bf16 values to
-// int8 59 us (3970), to q8_K with y 70 (4390), of 2048 rows of f32 32 (4490), quantized as
-// they are 20 (5000), combined by glu first 43 (3900).
+// rate of f32's. Measured (GB/s of what has to move; inputs from HBM, calls one behind the
+// other in a replayed graph, here and below): norm with the residual of 8192 rows of 4096 bf16
+// values to int8 56 to 59 us (4100), to q8_K with y 68 (4520), of 2048 rows of f32 to q8_K
+// with y 34 (4190); 8192 rows of bf16 quantized as they are 23 (4370), combined by glu first
+// 43 (3910).
 #include "pk_elem.h"
 #include "pk_epilogue.h"
 
@@ -158,7 +160,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs<TYPE> a) {
     const bool blocks = a.format == PULSAR_ROWS_Q8_K;
     auto first = [&](uint32_t j) { return V * (64u * (wave + waves * j) + lane); };
     // f of how many of the lane's values of chunk j are there: a constant where all lanes'
-    // are, whose loads then need no masks (2048 rows of 14336 f32 values 96 us against 104)
+    // are, whose loads then need no masks (2048 rows of 14336 f32 values to int8 97 us against
+    // 106)
     auto with_count = [&](uint32_t j, auto f) {
         if (64u * V * (wave + waves * j + 1u) <= a.dim)  // wave-uniform
             f(V);
@@ -531,11 +534,13 @@ struct RowShape {
     uint32_t waves, chunks;
 };
 // Few rows take as many waves as there are chunks (norm of one row of 4096 bf16 values
-// 4.3 us, with two chunks a wave 4.7). Many rows want fewer waves to start and more of a
+// 4.2 us, with two chunks a wave 4.5). Many rows want fewer waves to start and more of a
 // row on its way in each: two chunks (8192 rows of 4096 bf16 values, combined: 43 us, one
-// chunk 60), and twice as many where a row would take more than 12 waves, so that a CU
-// has room for a second (4096 rows of 14336 bf16 values combined 84 against 113, norm of
-// 4096 rows of 8192 f32 values 114 against 133; at 11 waves 81 against 79).
+// chunk 59; normed to int8 56 / 61), and twice as many where a row would take more than 12
+// waves, so that a CU has room for a second (4096 rows of 14336 bf16 values combined 84
+// against 113, quantized as they are 41 / 49; of 11264, 11 waves, combined 78 against 75). A
+// norm has gained nothing by the latter since its whole chunks have no masks (4096 rows of
+// 8192 f32 values to int8 87 / 85, to q8_K with y 114 / 111).
 static RowShape row_shape(uint32_t n_chunk, uint32_t n_rows, uint32_t most) {
     uint32_t nb = 1u;
     const bool few = n_rows < 256u || n_chunk == 1u;
@@ -544,8 +549,10 @@ static RowShape row_shape(uint32_t n_chunk, uint32_t n_rows, uint32_t most) {
     if (n_chunk > 16u * nb) return {16u, 0u};
     return {(n_chunk + nb - 1u) / nb, nb};
 }
-// Chunks of a wave at most: 16 values a lane in a norm, whose products are of 64 bits
-// (with 32, 2048 rows of 14336 f32 values took 151 us against 133), 32 in the quantizers
+// Chunks of a wave at most: 16 values a lane in a norm, whose products are of 64 bits, 32 in
+// the quantizers. With masks on its loads a norm was slower with 32 (2048 rows of 14336 f32
+// values 151 us against 133); since whole chunks have none, 32 takes 3% less (to int8 93 / 97,
+// to q8_K with y 120 / 124)
 template <uint32_t TYPE>
 constexpr uint32_t kNormChunks = 16u / kLane<TYPE>;
 template <uint32_t TYPE>
