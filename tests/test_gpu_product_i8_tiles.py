@@ -12,6 +12,7 @@ import torch
 from pulsar_amd import kernels as K
 from pulsar_amd import runtime
 from pulsar_amd.formats import EPI_GELU, EPI_NONE, EPI_RELU, EPI_SIGMOID, EPI_SILU, TYPE_BF16, TYPE_F16, TYPE_F32
+from tests.test_gpu_grouped_choice import launches
 from tests.test_gpu_rows8 import HALF, NAMES, TINY, TORCH
 
 pytestmark = pytest.mark.gpu
@@ -19,32 +20,12 @@ KINDS = [TYPE_F32, TYPE_F16, TYPE_BF16]
 ACTS = [EPI_SILU, EPI_GELU, EPI_RELU, EPI_SIGMOID, EPI_NONE]
 
 
-class KernelNode(ctypes.Structure):
-    """hipKernelNodeParams"""
-
-    _fields_ = [("block", ctypes.c_uint32 * 3), ("extra", ctypes.c_void_p), ("func", ctypes.c_void_p),
-                ("grid", ctypes.c_uint32 * 3), ("params", ctypes.c_void_p), ("shared", ctypes.c_uint32)]
-
-
 def kernel_of(call):
     """The name of the one kernel that a call launches (nothing runs)."""
-    hip, vp = runtime._hip(), ctypes.c_void_p
-    graph, count = vp(), ctypes.c_size_t()
-    runtime._check(hip.hipStreamBeginCapture(runtime.STREAM_PER_THREAD, runtime.CAPTURE_THREAD_LOCAL), "begin")
-    try:
-        call()
-    finally:
-        runtime._check(hip.hipStreamEndCapture(runtime.STREAM_PER_THREAD, ctypes.byref(graph)), "end")
-    try:
-        runtime._check(hip.hipGraphGetNodes(graph, None, ctypes.byref(count)), "count")
-        assert count.value == 1
-        nodes, node = (vp * 1)(), KernelNode()
-        runtime._check(hip.hipGraphGetNodes(graph, nodes, ctypes.byref(count)), "nodes")
-        runtime._check(hip.hipGraphKernelNodeGetParams(vp(nodes[0]), ctypes.byref(node)), "node")
-        hip.hipKernelNameRefByPtr.restype = ctypes.c_char_p
-        return hip.hipKernelNameRefByPtr(vp(node.func), vp(runtime.STREAM_PER_THREAD)).decode()
-    finally:
-        hip.hipGraphDestroy(graph)
+    node, = launches(call)
+    name = runtime._hip().hipKernelNameRefByPtr
+    name.argtypes, name.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_char_p
+    return name(node.func, runtime.STREAM_PER_THREAD).decode()
 
 
 def tile_of(name):
