@@ -350,7 +350,8 @@ extern "C" int pulsar_router_logits_q8(void *logits, void *xq, const void *x, co
     const uint32_t nb = (in_dim + 255u) / 256u;
     const uint64_t qblocks = ((uint64_t)n_tok * nb + 3u) / 4u;
     const uint64_t gemv_blocks = work;
-    if ((gemv_blocks + qblocks) >> 31) return reject("router logits q8 (size)");
+    // indices of 32 bits: of the blocks, and of their q8_K blocks, past the last ones too
+    if ((gemv_blocks + qblocks) >> 31 || (uint64_t)n_tok * nb > 0xffff0000ull) return reject("router logits q8 (size)");
     const dim3 grid = grid_of(gemv_blocks + qblocks);
     const uint32_t rbl = gemv_xcd_split(n_expert, (n_tok + tg - 1u) / tg, tg);
     if (tg == 1u)

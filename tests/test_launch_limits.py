@@ -78,6 +78,7 @@ def test_the_most_rows_reach_a_launch(capfd, call, rows):
     lambda: K.matmul_f32(A[0], A[1], A[2], 2**32 - 255, 1, 1), lambda: K.matmul_f32(A[0], A[1], A[2], 4, 1, 2**32 - 1),
     lambda: K.router_logits_q8(A[0], A[1], A[2], A[3], 0, 2**32 - 1, 1, 1),
     lambda: K.router_logits_q8(A[0], A[1], A[2], A[3], 0, 4, 1, 2**32 - 1),
+    lambda: K.router_logits_q8(A[0], A[1], A[2], A[3], 0, 1280, 1, 2**30),
     lambda: K.router_select(A[0], A[1], A[2], 0, 1, 1, 1.0, 2**31, 0, 0), lambda: K.add_bias_rows(A[0], A[1], 2**20, 2**19),
     lambda: K.moe_slot_sum(A[0], A[1], 2**20, 1, 2**19), lambda: K.moe_down_bias(A[0], A[1], A[2], 2**20, 1, 2**19),
     lambda: K.moe_slot_sum_bias(A[0], A[1], A[2], A[3], 2**20, 1, 2**19),
