@@ -175,9 +175,9 @@ int pulsar_rms_norm_q8(void *q, void *scales, void *y, void *sum, const void *x,
  * is given of v = glu(x, up, act_op), the gated combine of pulsar_moe_pair_swiglu in 64
  * bits (SWIGLU_OAI's alpha: 1.702). Gates far below 0 count as they stand, under
  * e^gate's end of the normal numbers too (the scale is 0 there); where it is below 2^-1074
- * for the whole row, about -745, the row is one of zeros. up NULL: act_op 0. gate and up may be columns of one
- * array. dim <= 2^24, n_rows < 2^31, strides < 2^32. q or scales over an input or one
- * another are refused. */
+ * for the whole row, about -745, the row is one of zeros. up NULL: act_op 0. gate and up
+ * may be columns of one array. dim <= 2^24, n_rows < 2^31, strides < 2^32. q or scales over
+ * an input or one another are refused. */
 int pulsar_quantize_i8(void *q, void *scales, const void *x, const void *up, uint32_t dim,
                        uint32_t n_rows, uint32_t act_op, uint32_t type, uint64_t x_stride,
                        uint64_t up_stride, uint64_t q_stride);
